@@ -430,3 +430,55 @@ def all(a, /, axis=None, out=None, keepdims=False, *, where=True):
 def any(a, /, axis=None, out=None, keepdims=False, *, where=True):
     check_limitations(where=where)
     return get_result_array(dpt.any(get_usm_ndarray(a), axis=axis, keepdims=keepdims), out)
+
+
+# ----------------------------------------------------------- row operators
+def _row_call(fn, arrays, out, **kwargs):
+    """A row operator of the tensor layer on public arrays: results are public arrays, an `out` array itself
+    where one was given (numbers and None among `arrays` pass through)."""
+    usm = [a if a is None or isinstance(a, (int, float, np.generic)) else get_usm_ndarray(a) for a in arrays]
+    several = isinstance(out, (tuple, list))
+    usm_out = type(out)(None if o is None else get_usm_ndarray(o) for o in out) if several \
+        else None if out is None else get_usm_ndarray(out)
+    res = fn(*usm, out=usm_out, **kwargs)
+    if not isinstance(res, tuple):
+        return _wrap(res) if out is None or isinstance(out, usm_ndarray) else out
+    given = out if several else (None,) * len(res)
+    return tuple(o if isinstance(o, dpnp_array) else _wrap(r) for o, r in zip(given, res))
+
+
+def layer_norm(x, weight=None, bias=None, /, *, axis=-1, eps=1e-5, return_stats=False, out=None):
+    return _row_call(dpt.layer_norm, (x, weight, bias), out, axis=axis, eps=eps, return_stats=return_stats)
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, /, *, axis=-1, weight_grads=True, out=None):
+    return _row_call(dpt.layer_norm_backward, (dy, x, mean, rstd, weight), out, axis=axis, weight_grads=weight_grads)
+
+
+def embedding(table, ids, /, *, scale=1.0, out=None):
+    return _row_call(dpt.embedding, (table, ids), out, scale=scale)
+
+
+def embedding_backward(dout, ids, num_rows, /, *, scale=1.0, dtype=None, out=None):
+    return _row_call(dpt.embedding_backward, (dout, ids, num_rows), out, scale=scale, dtype=dtype)
+
+
+def distillation_loss(logits, teacher_logits, teacher_index, /, *, temperature=1.0, return_stats=False, out=None):
+    return _row_call(dpt.distillation_loss, (logits, teacher_logits, teacher_index), out, temperature=temperature,
+                     return_stats=return_stats)
+
+
+def distillation_loss_backward(dloss, logits, teacher_logits, teacher_index, stats, /, *, temperature=1.0, out=None):
+    return _row_call(dpt.distillation_loss_backward, (dloss, logits, teacher_logits, teacher_index, stats), out,
+                     temperature=temperature)
+
+
+def distillation_loss_and_grad(logits, teacher_logits, teacher_index, dloss=1.0, /, *, temperature=1.0, out=None):
+    return _row_call(dpt.distillation_loss_and_grad, (logits, teacher_logits, teacher_index, dloss), out,
+                     temperature=temperature)
+
+
+for _f in (layer_norm, layer_norm_backward, embedding, embedding_backward, distillation_loss, distillation_loss_backward,
+           distillation_loss_and_grad):
+    _f.__doc__ = getattr(dpt, _f.__name__).__doc__
+del _f

@@ -156,6 +156,13 @@ PROTOTYPES = {
     "dpb_reduce_dtype_supported": (_i, [_i, _i, _i]),
     "dpb_reduction_over_axis": (_i, [_i, _parr, _i, _parr, _vp]),
     "dpb_search_over_axis": (_i, [_i, _parr, _i, _parr, _vp]),
+    "dpb_layer_norm": (_i, [_parr, _parr, _parr, _dbl, _parr, _parr, _parr, _vp]),
+    "dpb_layer_norm_backward": (_i, [_parr] * 8 + [_vp]),
+    "dpb_embedding": (_i, [_parr, _parr, _dbl, _parr, _vp]),
+    "dpb_embedding_backward": (_i, [_parr, _parr, _dbl, _parr, _vp]),
+    "dpb_distillation_loss": (_i, [_parr, _parr, _parr, _dbl, _parr, _parr, _vp]),
+    "dpb_distillation_loss_backward": (_i, [_parr] * 5 + [_dbl, _parr, _vp]),
+    "dpb_distillation_loss_and_grad": (_i, [_parr] * 4 + [_dbl, _parr, _parr, _vp]),
     "dpb_black_scholes_f64": (_i, [_i64, _vp, _vp, _vp, _dbl, _dbl, _vp, _vp, _vp]),
     "dpb_fused_elementwise": (_i, [_vp, _i64, _vp]),
     "dpb_fused_elementwise_specialized": (_i, [_vp, _i64, _vp]),

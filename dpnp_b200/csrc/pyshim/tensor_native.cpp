@@ -69,6 +69,9 @@ struct ArrayCore {
 
 inline void *as_stream(uintptr_t s) { return reinterpret_cast<void *>(s); }
 
+// an optional array: None arrives as a null pointer
+inline const dpb_array *maybe(const ArrayCore *a) { return a ? &a->d : nullptr; }
+
 inline void use_device(int device) { check(dpb_set_device(device)); }
 
 // One block of the stream-ordered pool; returned to the pool, ordered after the work already
@@ -171,6 +174,48 @@ PYBIND11_MODULE(_tensor_native, m, py::mod_gil_not_used())
                            uintptr_t stream) {
         use_device(dst.d.device);
         check(dpb_accumulate_over_axis(op, &src.d, &dst.d, include_initial, as_stream(stream)));
+    });
+    // row operators (_tensor_rows_impl); optional arrays are None
+    m.def("layer_norm", [](const ArrayCore &x, const ArrayCore *w, const ArrayCore *b, double eps, const ArrayCore &y,
+                           const ArrayCore *mean, const ArrayCore *rstd, uintptr_t stream) {
+        use_device(y.d.device);
+        check(dpb_layer_norm(&x.d, maybe(w), maybe(b), eps, &y.d, maybe(mean), maybe(rstd), as_stream(stream)));
+    });
+    m.def("layer_norm_backward", [](const ArrayCore &dy, const ArrayCore &x, const ArrayCore &mean, const ArrayCore &rstd,
+                                    const ArrayCore *w, const ArrayCore &dx, const ArrayCore *dw, const ArrayCore *db,
+                                    uintptr_t stream) {
+        use_device(dx.d.device);
+        check(dpb_layer_norm_backward(&dy.d, &x.d, &mean.d, &rstd.d, maybe(w), &dx.d, maybe(dw), maybe(db),
+                                      as_stream(stream)));
+    });
+    m.def("embedding", [](const ArrayCore &table, const ArrayCore &ids, double scale, const ArrayCore &out,
+                          uintptr_t stream) {
+        use_device(out.d.device);
+        check(dpb_embedding(&table.d, &ids.d, scale, &out.d, as_stream(stream)));
+    });
+    m.def("embedding_backward", [](const ArrayCore &dout, const ArrayCore &ids, double scale, const ArrayCore &dtable,
+                                   uintptr_t stream) {
+        use_device(dtable.d.device);
+        check(dpb_embedding_backward(&dout.d, &ids.d, scale, &dtable.d, as_stream(stream)));
+    });
+    m.def("distillation_loss", [](const ArrayCore &z, const ArrayCore &top, const ArrayCore &index, double temperature,
+                                  const ArrayCore &loss, const ArrayCore *stats, uintptr_t stream) {
+        use_device(loss.d.device);
+        check(dpb_distillation_loss(&z.d, &top.d, &index.d, temperature, &loss.d, maybe(stats), as_stream(stream)));
+    });
+    m.def("distillation_loss_backward", [](const ArrayCore &dloss, const ArrayCore &z, const ArrayCore &top,
+                                           const ArrayCore &index, const ArrayCore &stats, double temperature,
+                                           const ArrayCore &dz, uintptr_t stream) {
+        use_device(dz.d.device);
+        check(dpb_distillation_loss_backward(&dloss.d, &z.d, &top.d, &index.d, &stats.d, temperature, &dz.d,
+                                             as_stream(stream)));
+    });
+    m.def("distillation_loss_and_grad", [](const ArrayCore &z, const ArrayCore &top, const ArrayCore &index,
+                                           const ArrayCore &dloss, double temperature, const ArrayCore &loss,
+                                           const ArrayCore &dz, uintptr_t stream) {
+        use_device(dz.d.device);
+        check(dpb_distillation_loss_and_grad(&z.d, &top.d, &index.d, &dloss.d, temperature, &loss.d, &dz.d,
+                                             as_stream(stream)));
     });
     m.def("unary_result_type", &dpb_unary_result_type);
     m.def("binary_result_type", &dpb_binary_result_type);

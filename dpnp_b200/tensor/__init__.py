@@ -23,6 +23,8 @@ from ._manipulation_functions import (broadcast_arrays, broadcast_shapes, broadc
                                       flip, permute_dims, reshape, squeeze)
 from ._reduction import (all, any, argmax, argmin, count_nonzero, logsumexp, max, min, prod, reduce_hypot,
                          sum)
+from ._row_functions import (distillation_loss, distillation_loss_and_grad, distillation_loss_backward, embedding,
+                             embedding_backward, layer_norm, layer_norm_backward)
 from ._search_functions import where
 from ._accumulation import cumulative_logsumexp, cumulative_prod, cumulative_sum
 from ._statistical_functions import mean, std, var

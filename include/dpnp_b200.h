@@ -483,6 +483,57 @@ int dpb_accumulate_over_axis(int op, const dpb_array *src, const dpb_array *dst,
  * (_cumsum_over_axis_dtype_supported etc.). */
 int dpb_accumulate_dtype_supported(int op, int t_in, int t_out);
 
+/* ------------------------------------------------------- row operators   */
+/* Operators over the rows of a matrix that surround the matrix products of a language model: layer
+ * normalisation, embedding lookup, distillation from a teacher's top logits, and their gradients.  The
+ * reference has no counterpart; they extend its mean/var (dpnp/tensor/_statistical_functions.py:38-270)
+ * and logsumexp (dpnp/tensor/_reduction.py:515-577) families.
+ *
+ * Data is float16, float32 or float64; sums and statistics are float32 (float64 for float64 data:
+ * "the accumulation type" below) and every result is rounded once.  "Rows" are the leading axes of an
+ * array, in C order: the last axis has unit stride, the leading axes lie at most two strides apart
+ * after merging (a caller copies anything else).  At most 2^31 - 1 rows.  Outputs overlap no input,
+ * except where a result may be exactly the array it is computed from (in place).
+ * Errors: DPB_ERR_TYPE and DPB_ERR_VALUE for arguments, nothing is launched then.  All work is enqueued
+ * on `stream`; scratch comes from dpb_malloc on that stream, per call. */
+
+/* y = (x - mean) * rstd * weight + bias over the last axis, rstd = 1 / sqrt(var + eps).  weight, bias:
+ * one-dimensional, of the type of x or (float16 x) float32, or NULL; mean, rstd: C-contiguous, shape of
+ * the rows, accumulation type, or NULL.  y may be x. */
+int dpb_layer_norm(const dpb_array *x, const dpb_array *weight, const dpb_array *bias, double eps, const dpb_array *y,
+                   const dpb_array *mean, const dpb_array *rstd, void *stream);
+/* Gradients of dpb_layer_norm from its mean and rstd: dx, and (both or neither) dweight and dbias, which
+ * have the type of weight.  dx may be dy or x. */
+int dpb_layer_norm_backward(const dpb_array *dy, const dpb_array *x, const dpb_array *mean, const dpb_array *rstd,
+                            const dpb_array *weight, const dpb_array *dx, const dpb_array *dweight,
+                            const dpb_array *dbias, void *stream);
+
+/* out[i, :] = scale * table[ids[i], :]; rows of zeros for ids outside [0, rows of the table).  table:
+ * two-dimensional; ids: C-contiguous int32 or int64 of any shape; out: shape of ids, then the row. */
+int dpb_embedding(const dpb_array *table, const dpb_array *ids, double scale, const dpb_array *out, void *stream);
+/* dtable[v, :] = scale * sum of dout[i, :] over ids[i] == v, zeros for rows without an id; ids outside the
+ * table add nothing.  dtable has the type of dout or (float16 dout) float32.  The order of the sums is
+ * fixed: the same call gives the same bits. */
+int dpb_embedding_backward(const dpb_array *dout, const dpb_array *ids, double scale, const dpb_array *dtable, void *stream);
+
+/* Distillation.  logits: rows of V; teacher_logits (accumulation type) and teacher_index (int32 or int64):
+ * C-contiguous rows of K <= 1024 entries.  An entry counts when its index lies in [0, V) and its logit is
+ * above -inf; p = softmax(teacher_logits / T) over those, q = softmax(logits / T);
+ * loss = T^2 * sum p (log p - log q), 0 for a row without entries, whose logits are not read.
+ * stats (NULL, or shape of the rows + (2,), accumulation type): max of the row's logits and
+ * log sum exp((logits - max) / T), zeros for a row without entries. */
+int dpb_distillation_loss(const dpb_array *logits, const dpb_array *teacher_logits, const dpb_array *teacher_index,
+                          double temperature, const dpb_array *loss, const dpb_array *stats, void *stream);
+/* dlogits = dloss * T * (q - p) from the stats of dpb_distillation_loss; dloss: one value a row, or one
+ * value (no dimensions) for all.  dlogits may be logits. */
+int dpb_distillation_loss_backward(const dpb_array *dloss, const dpb_array *logits, const dpb_array *teacher_logits,
+                                   const dpb_array *teacher_index, const dpb_array *stats, double temperature,
+                                   const dpb_array *dlogits, void *stream);
+/* Both of the above in one call, for a dloss known beforehand (a weight per row, 1 / rows for the mean). */
+int dpb_distillation_loss_and_grad(const dpb_array *logits, const dpb_array *teacher_logits, const dpb_array *teacher_index,
+                                   const dpb_array *dloss, double temperature, const dpb_array *loss,
+                                   const dpb_array *dlogits, void *stream);
+
 /* ------------------------------------------------- fused expression paths */
 /* Black-Scholes call/put for n options in one pass (3 loads, 2 stores per
  * option): the expression chain of examples/example_bs.py:50-75 with every
