@@ -42,6 +42,22 @@ struct RowMap {
     }
 };
 
+// Walks rows r, r + step, r + 2 step, ... of an array: an addition a row where they are one stride apart.
+template <class T> struct RowWalk {
+    T *base, *p;
+    RowMap map;
+    int64_t delta;
+    DPB_D RowWalk(T *data, const RowMap &m, uint32_t r, uint32_t step)
+        : base(data), p(data + m(r)), map(m), delta(m.outer == 0 ? int64_t(step) * m.inner : 0)
+    {
+    }
+    DPB_D void next(uint32_t r)   // to row r, one step on (r < 2^31: the caller does not go beyond the last row)
+    {
+        if (map.outer == 0) p += delta;
+        else p = base + map(r);
+    }
+};
+
 // Host: rows of `a` (its leading nd-1 axes) as a RowMap; false when the last axis is not unit-stride
 // or the leading axes need more than two levels.
 inline bool make_row_map(const dpb_array &a, RowMap &map)
@@ -85,8 +101,46 @@ inline int row_vector(const void *p, const RowMap &map, int64_t width, int item,
     return v;
 }
 
+// The same for an operand that is read with the rows (a weight): its accesses are of 16 bytes at most.
+inline bool wide_ok(const void *p, int vec, int item)
+{
+    const int bytes = vec * item;
+    return !p || is_aligned(p, static_cast<size_t>(bytes > 16 ? 16 : bytes));
+}
+
+// launch_after_previous with dynamic shared memory.  A block of more than 48 KiB in all has to ask
+// for it.
+template <class... KArgs, class... Args>
+inline void launch_shared(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t shared, cudaStream_t stream, Args... args)
+{
+    if (shared > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    if (tuning_pdl()) {
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);   // an error stays in cudaGetLastError for check_launch
+}
+
 // -------------------------------------------------------------------------------- argument checks
 constexpr int64_t kMaxRows = INT32_MAX;   // row numbers are divided with 31-bit arithmetic
+
+// First element of an array and the one behind its last.
+inline void array_bounds(const dpb_array &a, const void *&lo, const void *&hi)
+{
+    int64_t first, last;
+    displacement_range(a, first, last);
+    const char *p = static_cast<const char *>(a.data);
+    lo = p + first * type_size(a.typenum);
+    hi = p + (last + 1) * type_size(a.typenum);
+}
 
 inline int64_t count_rows(const dpb_array &a)
 {
@@ -226,6 +280,46 @@ template <class F, class A> DPB_D A block_fold(F f, A v, A *buf)
     return v;
 }
 
+// R sums (R = 1, 2 or 4) over a warp (WARP) or over the whole block, the same bits in every thread.  The
+// first steps of the folds hand each half (quarter) of the warp one sum to go on with, which saves
+// shuffles; one barrier where there are several warps.  `buf` (32 R values, zeros where the block has no
+// warp) must not be the one of the previous call: slower threads may still be reading that.
+template <bool WARP, int R, class A> DPB_D void group_sums(A (&v)[R], A *buf)
+{
+    constexpr unsigned all = 0xffffffffu;
+    constexpr int part = 32 / R;   // lanes that share a sum
+    const int lane = threadIdx.x & 31;
+    A s = v[0];
+    if constexpr (R == 2) {
+        const bool low = lane < 16;
+        s = (low ? v[0] : v[1]) + __shfl_xor_sync(all, low ? v[1] : v[0], 16);
+    }
+    else if constexpr (R == 4) {
+        const bool low = lane < 16, even = (lane & 8) == 0;
+        const A p = (low ? v[0] : v[2]) + __shfl_xor_sync(all, low ? v[2] : v[0], 16);
+        const A q = (low ? v[1] : v[3]) + __shfl_xor_sync(all, low ? v[3] : v[1], 16);
+        s = (even ? p : q) + __shfl_xor_sync(all, even ? q : p, 8);
+    }
+#pragma unroll
+    for (int d = part / 2; d > 0; d >>= 1) s += __shfl_xor_sync(all, s, d);
+    if constexpr (!WARP) {
+        A *mine = buf + lane / part * 32;
+        const int at = lane & (part - 1);
+        if (at == 0) mine[threadIdx.x >> 5] = s;
+        __syncthreads();
+        s = mine[at];
+#pragma unroll
+        for (int k = part; k < 32; k += part) s += mine[k + at];
+#pragma unroll
+        for (int d = part / 2; d > 0; d >>= 1) s += __shfl_xor_sync(all, s, d);
+    }
+    if constexpr (R == 1) v[0] = s;
+    else {
+#pragma unroll
+        for (int k = 0; k < R; ++k) v[k] = __shfl_sync(all, s, k * part);
+    }
+}
+
 // fmaf / fma under the library's -fmad=false
 DPB_D float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 DPB_D double fma_(double a, double b, double c) { return fma(a, b, c); }
@@ -235,5 +329,276 @@ DPB_D float log_(float a) { return logf(a); }
 DPB_D double log_(double a) { return log(a); }
 DPB_D float sqrt_(float a) { return sqrtf(a); }
 DPB_D double sqrt_(double a) { return sqrt(a); }
+// 1 / sqrt(a): within 2 steps of float, 1 of double; a quotient and a root cost ten times the instructions
+DPB_D float rsqrt_(float a) { return rsqrtf(a); }
+DPB_D double rsqrt_(double a) { return rsqrt(a); }
+
+// ----------------------------------------------------------------------------- arrays in registers
+// Element-wise arithmetic on a thread's values.  float pairs go through the two-lane instructions
+// (add/mul/fma.rn.f32x2, each lane rounded as the scalar instruction rounds it), which halves the
+// number of instructions: with 16-bit data these kernels are otherwise bound by issue, not by memory.
+DPB_D float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
+DPB_D float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
+DPB_D float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
+          "l"(reinterpret_cast<unsigned long long &>(c)));
+    return r;
+}
+DPB_D double2 add2(double2 a, double2 b) { return make_double2(a.x + b.x, a.y + b.y); }
+DPB_D double2 mul2(double2 a, double2 b) { return make_double2(a.x * b.x, a.y * b.y); }
+DPB_D double2 fma2(double2 a, double2 b, double2 c) { return make_double2(fma(a.x, b.x, c.x), fma(a.y, b.y, c.y)); }
+template <class A> struct pair_of { using type = float2; };
+template <> struct pair_of<double> { using type = double2; };
+
+// N values as N / 2 pairs (N even) or single values.
+template <class A, int N> struct Values {
+    static constexpr bool paired = N % 2 == 0;
+    using P = std::conditional_t<paired, typename pair_of<A>::type, A>;
+    static constexpr int M = paired ? N / 2 : N;
+    P p[M];
+    static DPB_D P all(A s)
+    {
+        if constexpr (paired) return P{s, s};
+        else return s;
+    }
+    static DPB_D P add_(P a, P b)
+    {
+        if constexpr (paired) return add2(a, b);
+        else return a + b;
+    }
+    static DPB_D P mul_(P a, P b)
+    {
+        if constexpr (paired) return mul2(a, b);
+        else return a * b;
+    }
+    static DPB_D P fma3(P a, P b, P c)
+    {
+        if constexpr (paired) return fma2(a, b, c);
+        else return fma_(a, b, c);
+    }
+    DPB_D A get(int i) const
+    {
+        if constexpr (paired) return i & 1 ? p[i / 2].y : p[i / 2].x;
+        else return p[i];
+    }
+    DPB_D void set(int i, A v)
+    {
+        if constexpr (paired) (i & 1 ? p[i / 2].y : p[i / 2].x) = v;
+        else p[i] = v;
+    }
+    DPB_D void fill(A s)
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = all(s);
+    }
+    DPB_D void add(const Values &o)   // += o
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = add_(p[i], o.p[i]);
+    }
+    DPB_D void add(A s)
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = add_(p[i], all(s));
+    }
+    DPB_D void mul(const Values &o)
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = mul_(p[i], o.p[i]);
+    }
+    DPB_D void mul(A s)
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = mul_(p[i], all(s));
+    }
+    DPB_D void fma_add(const Values &a, const Values &b)   // += a b
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = fma3(a.p[i], b.p[i], p[i]);
+    }
+    DPB_D void fma_add(const Values &a, A s)   // += a s
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) p[i] = fma3(a.p[i], all(s), p[i]);
+    }
+    // sums that gather in one pair (one value): one instruction a pair, then a single addition
+    DPB_D void sum_into(P &s) const
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) s = add_(s, p[i]);
+    }
+    DPB_D void sum_into(P &s, A times) const
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) s = fma3(p[i], all(times), s);
+    }
+    DPB_D void dot_into(P &s, const Values &o) const
+    {
+#pragma unroll
+        for (int i = 0; i < M; ++i) s = fma3(p[i], o.p[i], s);
+    }
+    static DPB_D A join(P s)
+    {
+        if constexpr (paired) return s.x + s.y;
+        else return s;
+    }
+};
+
+// VEC stored elements to numbers of the accumulation type and back (each rounded once).
+template <class A, int N, class T> DPB_D void unpack(const vec_t<T, N> &v, Values<A, N> &out)
+{
+    if constexpr (is_half_v<T> && N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) out.p[i / 2] = __half22float2(*reinterpret_cast<const __half2 *>(v.v + i));
+    }
+    else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out.set(i, to_acc<A>(v.v[i]));
+    }
+}
+template <class T, int N, class A> DPB_D vec_t<T, N> repack(const Values<A, N> &in)
+{
+    vec_t<T, N> v;
+    if constexpr (is_half_v<T> && N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2)
+            *reinterpret_cast<__half2 *>(v.v + i) = __float22half2_rn(in.p[i / 2]);
+    }
+    else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v.v[i] = from_acc<T>(in.get(i));
+    }
+    return v;
+}
+
+// N elements at p (aligned to the accesses, which are of at most 16 bytes), through the read-only path:
+// for arrays that the kernel does not write.
+template <class A, int N, class W> DPB_D void load_values(const W *p, Values<A, N> &out)
+{
+    constexpr int part = N * sizeof(W) > 16 ? 16 / static_cast<int>(sizeof(W)) : N;
+#pragma unroll
+    for (int k = 0; k < N; k += part) {
+        Values<A, part> some;
+        unpack<A, part, W>(load_vec<vec_t<W, part>>(p + k), some);
+#pragma unroll
+        for (int j = 0; j < part; ++j) out.set(k + j, some.get(j));
+    }
+}
+
+// ------------------------------------------------------------------- rows fetched ahead into shared memory
+// Copy of one access (16, 8 or 4 bytes) into shared memory that does not wait (2 bytes: a plain copy).
+template <class V> DPB_D void copy_async(V *shared, const V *global)
+{
+    if constexpr (sizeof(V) == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared))),
+                     "l"(global)
+                     : "memory");
+    else if constexpr (sizeof(V) >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared))),
+                     "l"(global), "n"(sizeof(V))
+                     : "memory");
+    else *shared = *global;
+}
+DPB_D void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> DPB_D void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The accesses of one thread to a row of n elements: ITEMS accesses of VEC elements, `width` threads apart.
+// Where a row starts `mis` elements behind a 16-byte boundary the accesses start at that boundary (the
+// columns are shifted by mis), so that every access is aligned; the first and the last then reach into
+// the neighbouring rows, which is read (and not used) where it lies inside the array, and go element by
+// element at the array's ends.  SHIFT = false: every row is aligned and n is a multiple of VEC.
+template <class T, int VEC, int ITEMS, bool SHIFT> struct RowAccess {
+    using V = vec_t<T, VEC>;
+    int t, width, n, mis;
+    DPB_D int column(int i) const { return (i * width + t) * VEC - (SHIFT ? mis : 0); }
+    DPB_D bool any(int i) const { return column(i) < n && (!SHIFT || column(i) > -VEC); }
+    DPB_D bool whole(int i) const { return !SHIFT || (column(i) >= 0 && column(i) + VEC <= n); }
+    DPB_D bool has(int i, int j) const { return column(i) + j >= 0 && column(i) + j < n; }
+    // zeros in the slots that no fetch will fill, for `rows` rows of the ring
+    DPB_D void clear(V *slot, int stride, int rows) const
+    {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (any(i)) continue;
+            V v;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v.v[j] = from_acc<T>(acc_t<T>(0));
+            for (int k = 0; k < rows; ++k) slot[(k * ITEMS + i) * stride] = v;
+        }
+    }
+    // into the thread's own slots of shared memory, `stride` accesses apart; [lo, hi): the array
+    DPB_D void fetch(const T *row, V *slot, int stride, const T *lo, const T *hi) const
+    {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (!any(i)) continue;
+            const T *p = row + column(i);
+            if (whole(i) || (p >= lo && p + VEC <= hi)) copy_async(slot + i * stride, reinterpret_cast<const V *>(p));
+            else {
+                V v;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (has(i, j)) v.v[j] = p[j];
+                slot[i * stride] = v;
+            }
+        }
+    }
+    // zeros in place of what is not in the row
+    template <class A> DPB_D void clip(int i, Values<A, VEC> &v) const
+    {
+        if (whole(i)) return;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (!has(i, j)) v.set(j, A(0));
+    }
+    // `aligned`: this row lies on the boundaries that the columns were shifted for
+    DPB_D void store(T *row, int i, const V &v, bool aligned) const
+    {
+        T *p = row + column(i);
+        if (whole(i) && (!SHIFT || aligned)) {
+            *reinterpret_cast<V *>(p) = v;
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (has(i, j)) p[j] = v.v[j];
+    }
+    // values of an array of n elements that goes with the columns (a weight); `otherwise` outside
+    template <class A, class W> DPB_D void load(const W *w, int i, Values<A, VEC> &out, A otherwise) const
+    {
+        out.fill(otherwise);
+        if (!w || !any(i)) return;
+        if constexpr (!SHIFT) load_values<A, VEC, W>(w + column(i), out);
+        else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (has(i, j)) out.set(j, to_acc<A>(w[column(i) + j]));
+        }
+    }
+};
+
+// Elements between the 16-byte boundary below p and p.
+template <class T> DPB_D int misalignment(const T *p)
+{
+    return static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16) / static_cast<int>(sizeof(T));
+}
 
 }  // namespace dpb

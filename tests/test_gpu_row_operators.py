@@ -262,13 +262,15 @@ def test_layer_norm_out_and_in_place(dt, n):
     big = dp.zeros((11, n + 5), dtype=dt)
     m2, r2 = dp.empty(11, dtype=ACC[dt]), dp.empty(11, dtype=ACC[dt])
     res = dp.layer_norm(dev(x), dev(w), dev(b), return_stats=True, out=(big[:, 3:n + 3], m2, r2))
-    assert res[1] is m2 and np.array_equal(host(big)[:, 3:n + 3], host(y)) and np.array_equal(host(r2), host(rstd))
+    # rows that start elsewhere may be read in narrower accesses, and the sums then run in another order
+    assert res[1] is m2
+    check_norm(x, w, b, 1e-5, host(big)[:, 3:n + 3], host(m2), host(r2))
     assert not host(big)[:, :3].any() and not host(big)[:, n + 3:].any()
     d = dev(x)
     assert dp.layer_norm(d, dev(w), dev(b), out=d) is d and np.array_equal(host(d), host(y))
     d = dev(np.concatenate([x.ravel(), x.ravel()[:1]]))               # shifted by one element: a partial overlap
     dp.layer_norm(d[:-1].reshape(11, n), dev(w), dev(b), out=d[1:].reshape(11, n))
-    assert np.array_equal(host(d)[1:].reshape(11, n), host(y))
+    check_norm(x, w, b, 1e-5, host(d)[1:].reshape(11, n), host(mean), host(rstd))
     want = [host(t) for t in dp.layer_norm_backward(dev(dy), dev(x), mean, rstd, dev(w))]
     for over in (0, 1):
         p = [dev(dy), dev(x)]
