@@ -254,163 +254,226 @@ __global__ void __launch_bounds__(kThreads) layer_norm_columns_kernel(const T *d
     part[(int64_t(blockIdx.y) * 2 + 1) * n + c] = db;
 }
 
-// One pass over dy and x for all three gradients.  A block (TPR = 32: each of its 8 warps) takes every
-// gridDim-th row; its threads own fixed columns, so that dw and db gather in registers over all rows of the
-// block and only one partial sum a block goes through memory.  The next row's loads are issued before the
-// current row's two sums are folded (one barrier a row, two buffers in turn).
-template <class T, class W, int VEC, int TPR, int ITEMS>
-__global__ void __launch_bounds__(TPR < 256 ? (TPR == 32 ? 256 : TPR) : TPR, TPR >= 1024 ? 1 : TPR == 512 ? 2 : 3)
-    layer_norm_backward_kernel(const T *dy, RowMap dym, const T *x, RowMap xm, const acc_t<T> *mean, const acc_t<T> *rstd,
-                               const W *w, T *dx, RowMap dxm, acc_t<T> *part, int64_t rows, int n)
+// One pass over dy and x for all three gradients.  The threads of a group own fixed columns, so that dw and
+// db gather in registers over all rows of the group and one partial sum a block goes through memory; the
+// rows travel through shared memory as in layer_norm_kernel.  HOLD: the products of the first sweep (dy w
+// and h) stay in registers for the second and the ring has one slot; otherwise they are formed again from
+// the ring.
+template <class T, class W, int VEC, int ITEMS, bool WARP, int R, int DEPTH, bool HOLD, bool SHIFT, int THREADS>
+__global__ void __launch_bounds__(WARP ? 256 : THREADS, WARP ? THREADS / 256 : 1)
+    layer_norm_backward_kernel(const T *dy, RowMap dym, Span<T> dys, const T *x, RowMap xm, Span<T> xs, const acc_t<T> *mean,
+                               const acc_t<T> *rstd, const W *w, T *dx, RowMap dxm, acc_t<T> *part, uint32_t rows, int n)
 {
+    static_assert(HOLD || DEPTH > 1, "the second sweep reads the ring");
     using A = acc_t<T>;
     using V = vec_t<T, VEC>;
-    constexpr int groups = TPR == 32 ? 8 : 1;
-    __shared__ A buf[2][64];
-    extern __shared__ char dynamic[];
-    for (int i = threadIdx.x; i < 128; i += blockDim.x) (&buf[0][0])[i] = 0;
-    __syncthreads();
+    using Vals = Values<A, VEC>;
+    constexpr int groups = WARP ? 8 : 1;
+    const int threads = WARP ? 256 : blockDim.x;
+    extern __shared__ __align__(16) char shared_bytes[];
+    __shared__ A buf[2][32 * 2 * R];
+    if constexpr (!WARP) {
+        for (int i = threadIdx.x; i < 2 * 32 * 2 * R; i += threads) (&buf[0][0])[i] = 0;
+        __syncthreads();
+    }
     cudaGridDependencySynchronize();
-    const int t = threadIdx.x % TPR, group = TPR == 32 ? threadIdx.x / 32 : 0;
-    const int64_t step = int64_t(gridDim.x) * groups;
-    const A inv_n = A(1) / A(n);
-    Values<A, VEC> dw[ITEMS], db[ITEMS];
+    const uint32_t step = gridDim.x * groups;
+    uint32_t r = blockIdx.x * groups + (WARP ? threadIdx.x / 32 : 0);
+    const uint32_t first = r < rows ? r : 0;
+    const RowAccess<T, VEC, ITEMS, SHIFT> at = {static_cast<int>(WARP ? threadIdx.x & 31 : threadIdx.x), WARP ? 32 : threads, n,
+                                                SHIFT ? misalignment(x + xm(first)) : 0};
+    V *slot = reinterpret_cast<V *>(shared_bytes) + threadIdx.x;   // [DEPTH][R][dy, x][ITEMS][threads]
+    at.clear(slot, threads, DEPTH * R * 2);
+    RowWalk<const T> gw(dy, dym, first, step), xw(x, xm, first, step);
+    RowWalk<T> ow(dx, dxm, first, step);
+    uint32_t ahead = r;
+    const auto fetch = [&](int to) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            if (ahead >= rows) break;
+            at.fetch(gw.p, slot + ((to * R + k) * 2) * ITEMS * threads, threads, dys.lo, dys.hi);
+            at.fetch(xw.p, slot + ((to * R + k) * 2 + 1) * ITEMS * threads, threads, xs.lo, xs.hi);
+            ahead += step;
+            if (ahead < rows) {
+                gw.next(ahead);
+                xw.next(ahead);
+            }
+        }
+        copy_async_commit();
+    };
+    if constexpr (DEPTH == 1) fetch(0);
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
+    using Kept = KeptWeights<W, VEC, ITEMS>;
+    const Kept kept = {reinterpret_cast<typename Kept::S *>(shared_bytes + size_t(DEPTH) * R * 2 * ITEMS * threads * sizeof(V)) +
+                           threadIdx.x,
+                       threads};
+    kept.fill(0, w, at, 1.0f);
+    bool edge[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) edge[i] = SHIFT && __any_sync(0xffffffffu, at.any(i) && !at.whole(i));
+    Vals dw[ITEMS], db[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         dw[i].fill(0);
         db[i].fill(0);
     }
-    V g[ITEMS], v[ITEMS];
-    A m = 0, rs = 0;
-    int64_t r = int64_t(blockIdx.x) * groups + group;
-    const auto fetch = [&](int64_t row, V(&gg)[ITEMS], V(&vv)[ITEMS], A &mm, A &rr) {
-        const T *gr = dy + dym(static_cast<uint32_t>(row)), *xr = x + xm(static_cast<uint32_t>(row));
+    const A inv_n = A(1) / A(n);
+    int turn = 0, fold = 0;
+    A m_next[R], rs_next[R];
+    const auto statistics = [&](uint32_t from) {   // of the next round's rows, ahead of their use
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int c = (i * TPR + t) * VEC;
-            if (c >= n) continue;
-            gg[i] = *reinterpret_cast<const V *>(gr + c);
-            vv[i] = *reinterpret_cast<const V *>(xr + c);
+        for (int k = 0; k < R; ++k) {
+            const uint32_t row = min(from + k * step, rows - 1);
+            m_next[k] = mean[row];
+            rs_next[k] = rstd[row];
         }
-        mm = mean[row];
-        rr = rstd[row];
     };
-    if (r < rows) fetch(r, g, v, m, rs);
-    int turn = 0;
-    for (; r < rows; r += step) {
-        V g2[ITEMS], v2[ITEMS];
-        A m2 = 0, rs2 = 0;
-        if (r + step < rows) fetch(r + step, g2, v2, m2, rs2);
-        Values<A, VEC> a[ITEMS], h[ITEMS];
-        auto sum1 = Values<A, VEC>::all(0), sum2 = sum1;
+    statistics(r);
+    while (r < rows) {
+        if constexpr (DEPTH > 1) fetch(turn == 0 ? DEPTH - 1 : turn - 1);
+        A m[R], rs[R], s[2 * R];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int c = (i * TPR + t) * VEC;
-            if (c >= n) continue;
-            unpack<A, VEC, T>(v[i], h[i]);
-            unpack<A, VEC, T>(g[i], a[i]);
-            h[i].add(-m);
-            h[i].mul(rs);
-            dw[i].fma_add(a[i], h[i]);
-            db[i].add(a[i]);
-            if (w) {
-                Values<A, VEC> u;
-                load_values<A, VEC, W>(w + c, u);
-                a[i].mul(u);
-            }
-            if constexpr (is_half_v<T>) {
-                a[i].sum_into(sum1);
-                a[i].dot_into(sum2, h[i]);
-            }
-            else {
-                Values<A, VEC> u = a[i];
-                u.mul(inv_n);
-                u.sum_into(sum1);
-                u.dot_into(sum2, h[i]);
-            }
+        for (int k = 0; k < R; ++k) {
+            m[k] = m_next[k];
+            rs[k] = rs_next[k];
         }
-        A s1 = Values<A, VEC>::join(sum1), s2 = Values<A, VEC>::join(sum2);
-        A both[2] = {s1, s2};
-        group_sums<TPR == 32>(both, buf[turn]);
-        s1 = both[0];
-        s2 = both[1];
-        turn ^= 1;
-        if constexpr (is_half_v<T>) {
-            s1 *= inv_n;
-            s2 *= inv_n;
-        }
-        T *o = dx + dxm(static_cast<uint32_t>(r));
+        statistics(r + R * step);
+        copy_async_wait<DEPTH - 1>();
+        Vals a[HOLD ? R : 1][ITEMS], h[HOLD ? R : 1][ITEMS];
+        // dy and h of a row from the ring
+        const auto load = [&](int k, int i, Vals &aa, Vals &hh) {
+            unpack<A, VEC, T>(slot[((turn * R + k) * 2 * ITEMS + i) * threads], aa);
+            unpack<A, VEC, T>(slot[(((turn * R + k) * 2 + 1) * ITEMS + i) * threads], hh);
+            hh.add(-m[k]);
+            hh.mul(rs[k]);
+            if (SHIFT && edge[i]) {
+                at.clip(i, aa);
+                at.clip(i, hh);
+            }
+        };
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int c = (i * TPR + t) * VEC;
-            if (c >= n) continue;
-            a[i].add(-s1);
-            a[i].fma_add(h[i], -s2);
-            a[i].mul(rs);
-            *reinterpret_cast<V *>(o + c) = repack<T, VEC, A>(a[i]);
-        }
+        for (int k = 0; k < R; ++k) {
+            s[2 * k] = s[2 * k + 1] = 0;
+            if (r + k * step >= rows) continue;   // nothing of the ring's older rows goes into dw and db
+            auto sum1 = Vals::all(0), sum2 = sum1;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            g[i] = g2[i];
-            v[i] = v2[i];
+            for (int i = 0; i < ITEMS; ++i) {
+                Vals &aa = a[HOLD ? k : 0][i], &hh = h[HOLD ? k : 0][i], ww;
+                load(k, i, aa, hh);
+                dw[i].fma_add(aa, hh);
+                db[i].add(aa);
+                kept.get(0, i, ww);
+                aa.mul(ww);
+                if constexpr (is_half_v<T>) {
+                    aa.sum_into(sum1);
+                    aa.dot_into(sum2, hh);
+                }
+                else {
+                    Vals u = aa;
+                    u.mul(inv_n);
+                    u.sum_into(sum1);
+                    u.dot_into(sum2, hh);
+                }
+            }
+            s[2 * k] = Vals::join(sum1);
+            s[2 * k + 1] = Vals::join(sum2);
         }
-        m = m2;
-        rs = rs2;
+        if constexpr (DEPTH == 1) fetch(0);   // the rows are in registers now
+        group_sums<WARP>(s, buf[fold]);
+        fold ^= 1;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            if (r >= rows) break;
+            const A s1 = is_half_v<T> ? s[2 * k] * inv_n : s[2 * k], s2 = is_half_v<T> ? s[2 * k + 1] * inv_n : s[2 * k + 1];
+            const bool aligned = !SHIFT || misalignment(ow.p) == at.mis;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                if (!at.any(i)) continue;
+                Vals &aa = a[HOLD ? k : 0][i], &hh = h[HOLD ? k : 0][i];
+                if constexpr (!HOLD) {
+                    Vals ww;
+                    load(k, i, aa, hh);
+                    kept.get(0, i, ww);
+                    aa.mul(ww);
+                }
+                aa.add(-s1);
+                aa.fma_add(hh, -s2);
+                aa.mul(rs[k]);
+                at.store(ow.p, i, repack<T, VEC, A>(aa), aligned);
+            }
+            r += step;
+            if (r < rows) ow.next(r);
+        }
+        turn = turn == DEPTH - 1 ? 0 : turn + 1;
     }
     if (!part) return;
     part += int64_t(blockIdx.x) * 2 * n;
-    if constexpr (TPR == 32) {
-        // the warps' sums, added in the order of the warps
-        A *sum = reinterpret_cast<A *>(dynamic);
+    if constexpr (WARP) {
+        // the warps' sums, added in the order of the warps, over what was the ring
+        copy_async_wait<0>();
+        A *sum = reinterpret_cast<A *>(shared_bytes);
         for (int k = 0; k < groups; ++k) {
-            if (k == group) {
-#pragma unroll
-                for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const int c = (i * 32 + t) * VEC + j;
-                        if (c >= n) continue;
-                        sum[c] = k ? sum[c] + dw[i].get(j) : dw[i].get(j);
-                        sum[n + c] = k ? sum[n + c] + db[i].get(j) : db[i].get(j);
-                    }
-            }
             __syncthreads();
+            if (k != threadIdx.x / 32) continue;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const int c = at.column(i) + j;
+                    if (!at.has(i, j)) continue;
+                    sum[c] = k ? sum[c] + dw[i].get(j) : dw[i].get(j);
+                    sum[n + c] = k ? sum[n + c] + db[i].get(j) : db[i].get(j);
+                }
         }
-        for (int c = threadIdx.x; c < 2 * n; c += blockDim.x) part[c] = sum[c];
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * n; c += threads) part[c] = sum[c];
     }
     else {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const int c = (i * TPR + t) * VEC + j;
-                if (c >= n) continue;
+                const int c = at.column(i) + j;
+                if (!at.has(i, j)) continue;
                 part[c] = dw[i].get(j);
                 part[n + c] = db[i].get(j);
             }
     }
 }
 
-// dw, db = sum of the partial sums: 32 columns a block, 32 threads a column that take every 32nd partial
-// sum and are then added in order.
+// dw, db = sum of the partial sums: 64 columns a block, 32 threads a pair of columns that take every 32nd
+// partial sum and are then added in order.
 template <class A, class W>
 __global__ void __launch_bounds__(1024) layer_norm_join_kernel(const A *part, int64_t slabs, int64_t n, W *dw, W *db)
 {
-    __shared__ A buf[32][33];
+    using P = typename pair_of<A>::type;
+    __shared__ P buf[32][32];
     cudaGridDependencySynchronize();
     const int col = threadIdx.x & 31, lane = threadIdx.x >> 5;
-    const int64_t i = int64_t(blockIdx.x) * 32 + col;
-    A s = 0;
-    if (i < 2 * n)
-        for (int64_t k = lane; k < slabs; k += 32) s += part[k * 2 * n + i];
+    const int64_t i = (int64_t(blockIdx.x) * 32 + col) * 2;   // 2 n columns: pairs are whole and aligned
+    P s = {0, 0};
+    if (i < 2 * n) {
+        const int64_t jump = 32 * n;   // pairs
+        const P *p = reinterpret_cast<const P *>(part + lane * 2 * n + i);
+        int64_t k = lane;
+        for (; k + 7 * 32 < slabs; k += 8 * 32, p += 8 * jump) {   // eight loads in flight
+            P v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = p[u * jump];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s = add2(s, v[u]);
+        }
+        for (; k < slabs; k += 32, p += jump) s = add2(s, *p);
+    }
     buf[lane][col] = s;
     __syncthreads();
     if (lane > 0 || i >= 2 * n) return;
-    s = buf[0][col];
 #pragma unroll
-    for (int k = 1; k < 32; ++k) s += buf[k][col];
-    if (i < n) dw[i] = from_acc<W>(s);
-    else db[i - n] = from_acc<W>(s);
+    for (int k = 1; k < 32; ++k) s = add2(s, buf[k][col]);
+    const auto put = [&](int64_t c, A v) { (c < n ? dw[c] : db[c - n]) = from_acc<W>(v); };
+    put(i, s.x);
+    put(i + 1, s.y);
 }
 
 template <class T, class W>
@@ -449,15 +512,16 @@ struct NormArgs {
     double eps;
 };
 
-// As many blocks as the SMs hold at once (limited by threads and by shared memory).  Shifted rows: a
-// group's rows have to start at one and the same misalignment, which a step of a multiple of 16 bytes'
-// elements gives for rows one stride apart.
-static unsigned block_count(int64_t rows, int groups, int threads, size_t shared, bool shift)
+// As many blocks as the SMs hold at once (limited by threads and by shared memory), but at least `rounds`
+// rows a group.  Shifted rows: a group's rows have to start at one and the same misalignment, which a step
+// of a multiple of 16 bytes' elements gives for rows one stride apart.
+static unsigned block_count(int64_t rows, int groups, int rounds, int threads, size_t shared, bool shift, int an_sm_threads)
 {
-    const int64_t an_sm = std::max<int64_t>(1, std::min<int64_t>(kGroupThreads / threads, (227 * 1024) / int64_t(shared + 2048)));
-    const int64_t blocks = device_props().sm_count * an_sm;
-    if (rows <= blocks * groups) return static_cast<unsigned>(ceil_div(rows, groups));
-    return static_cast<unsigned>(shift ? std::max<int64_t>(blocks / 8 * 8, 8) : blocks);
+    const int64_t an_sm = std::max<int64_t>(1, std::min<int64_t>(an_sm_threads / threads, (227 * 1024) / int64_t(shared + 2048)));
+    const int64_t most = device_props().sm_count * an_sm;
+    int64_t blocks = std::min(most, ceil_div(rows, int64_t(groups) * rounds));
+    if (shift && blocks * groups < rows) blocks = blocks < 8 ? 8 : blocks / 8 * 8;
+    return static_cast<unsigned>(blocks);
 }
 
 // The elements of x for accesses that reach beyond a row; none when the rows are being overwritten.
@@ -475,7 +539,7 @@ static bool launch_forward(const NormArgs &a, int64_t accesses, cudaStream_t s)
     const int groups = WARP ? 8 : 1, threads = WARP ? 256 : static_cast<int>(ceil_div(ceil_div(accesses, ITEMS), 32) * 32);
     const size_t shared = size_t(DEPTH) * R * ITEMS * threads * sizeof(T) * VEC +
                           (KEEP == kShared ? KeptWeights<W, VEC, ITEMS>::bytes(threads) : 0);
-    launch_shared(layer_norm_kernel<T, W, VEC, ITEMS, WARP, R, DEPTH, KEEP, SHIFT>, block_count(a.rows, groups, threads, shared, SHIFT),
+    launch_shared(layer_norm_kernel<T, W, VEC, ITEMS, WARP, R, DEPTH, KEEP, SHIFT>, block_count(a.rows, groups, 1, threads, shared, SHIFT, kGroupThreads),
                   unsigned(threads), shared, s, static_cast<const T *>(a.x->data), a.xm, row_neighbours<T>(*a.x, *a.y),
                   a.w ? static_cast<const W *>(a.w->data) : nullptr, a.b ? static_cast<const W *>(a.b->data) : nullptr,
                   A(a.eps), static_cast<T *>(a.y->data), a.ym, a.mean ? static_cast<A *>(a.mean->data) : nullptr,
@@ -535,39 +599,27 @@ struct NormGradArgs {
 
 template <class T, class W> static int join_partials(const NormGradArgs &a, const acc_t<T> *part, int64_t slabs, cudaStream_t s)
 {
-    launch_after_previous(layer_norm_join_kernel<acc_t<T>, W>, static_cast<unsigned>(ceil_div(2 * a.n, 32)), 1024u, s, part,
+    launch_after_previous(layer_norm_join_kernel<acc_t<T>, W>, static_cast<unsigned>(ceil_div(a.n, 32)), 1024u, s, part,
                           slabs, a.n, static_cast<W *>(a.dw->data), static_cast<W *>(a.db->data));
     note_kernel("layer_norm_join");
     return check_launch("layer_norm_join");
 }
 
-template <class T, class W, int VEC, int TPR, int ITEMS>
-static int launch_backward(const NormGradArgs &a, cudaStream_t s)
+template <class T, class W, int VEC, int ITEMS, bool WARP, int R, int DEPTH, bool HOLD, bool SHIFT, int THREADS>
+static int launch_backward(const NormGradArgs &a, int64_t accesses, cudaStream_t s)
 {
     using A = acc_t<T>;
-    constexpr int groups = TPR == 32 ? 8 : 1, threads = TPR * groups;
-    // as many blocks as the SMs hold at once (1024 threads each), but at least two rows a block
-    const int64_t most = int64_t(device_props().sm_count) * (1024 / threads);
-    const int64_t blocks = std::max<int64_t>(1, std::min(most, ceil_div(a.rows, 2 * groups)));
+    const int groups = WARP ? 8 : 1, threads = WARP ? 256 : static_cast<int>(ceil_div(ceil_div(accesses, ITEMS), 32) * 32);
+    // (half of what KeptWeights keeps: there is no bias)
+    const size_t shared = size_t(DEPTH) * R * 2 * ITEMS * threads * sizeof(T) * VEC + KeptWeights<W, VEC, ITEMS>::bytes(threads) / 2;
+    const unsigned blocks = block_count(a.rows, groups, R, threads, shared, SHIFT, THREADS);
     void *part = nullptr;
-    if (a.dw) DPB_TRY(dpb_malloc(static_cast<size_t>(blocks * 2 * a.n) * sizeof(A), s, &part));
-    const size_t shared = TPR == 32 ? static_cast<size_t>(2 * a.n) * sizeof(A) : 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = shared;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    if (tuning_pdl()) {
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-    }
-    cudaLaunchKernelEx(&cfg, layer_norm_backward_kernel<T, W, VEC, TPR, ITEMS>, static_cast<const T *>(a.dy->data), a.dym,
-                       static_cast<const T *>(a.x->data), a.xm, static_cast<const A *>(a.mean->data),
-                       static_cast<const A *>(a.rstd->data), a.w ? static_cast<const W *>(a.w->data) : nullptr,
-                       static_cast<T *>(a.dx->data), a.dxm, static_cast<A *>(part), a.rows, static_cast<int>(a.n));
+    if (a.dw) DPB_TRY(dpb_malloc(static_cast<size_t>(int64_t(blocks) * 2 * a.n) * sizeof(A), s, &part));
+    launch_shared(layer_norm_backward_kernel<T, W, VEC, ITEMS, WARP, R, DEPTH, HOLD, SHIFT, THREADS>, blocks, unsigned(threads), shared, s,
+                  static_cast<const T *>(a.dy->data), a.dym, row_neighbours<T>(*a.dy, *a.dx),
+                  static_cast<const T *>(a.x->data), a.xm, row_neighbours<T>(*a.x, *a.dx), static_cast<const A *>(a.mean->data),
+                  static_cast<const A *>(a.rstd->data), a.w ? static_cast<const W *>(a.w->data) : nullptr,
+                  static_cast<T *>(a.dx->data), a.dxm, static_cast<A *>(part), static_cast<uint32_t>(a.rows), static_cast<int>(a.n));
     note_kernel("layer_norm_backward");
     int st = check_launch("layer_norm_backward");
     if (part) {
@@ -577,32 +629,43 @@ static int launch_backward(const NormGradArgs &a, cudaStream_t s)
     return st;
 }
 
-// Accumulators for dw and db and two rows' data: up to 8 columns a thread stay clear of spills at two
-// blocks of 512 threads an SM, 16 at one block of 1024.  False: the row is too long for that.
-template <class T, class W, int VEC> static bool run_rows_backward(const NormGradArgs &a, cudaStream_t s, int &st)
+// Measured at 16384 x 4096 float16 with float32 weights and 8192 x 4096 float32 (us):
+//   1024 threads an SM, one access, one row:  97 / 78; two rows: 105 / 76;
+//   512 threads an SM, two accesses, one row: 95 / 82; two rows: 96 / 74 (92 / 74 at 2048 columns).
+// More accesses a thread cost fewer instructions around the folds, fewer threads leave 128 registers for the
+// accumulators.  Shifted rows of float16 need registers for the edges too: one row, 640 threads.
+// False: the row is too long (then the columns are summed by a second pass over dy and x).
+template <class T, class W, int VEC, bool SHIFT> static bool run_rows_backward(const NormGradArgs &a, cudaStream_t s, int &st)
 {
-    const int64_t nv = ceil_div(a.n, VEC);
-#define DPB_ROWS(TPR, ITEMS) \
-    if (nv <= TPR * ITEMS) return st = launch_backward<T, W, VEC, TPR, ITEMS>(a, s), true;
+    const int64_t nv = ceil_div(a.n + (SHIFT ? VEC - 1 : 0), VEC);
+#define DPB_BACK(LIMIT, ITEMS, WARP, R, DEPTH, HOLD, THREADS)                                                       \
+    if (nv <= (LIMIT)) {                                                                                            \
+        st = launch_backward<T, W, VEC, ITEMS, WARP, R, DEPTH, HOLD, SHIFT, THREADS>(a, nv, s);                     \
+        return true;                                                                                                \
+    }
     if constexpr (VEC == 1) {
-        DPB_ROWS(32, 1)
-        DPB_ROWS(32, 4)
-        DPB_ROWS(128, 2)
-        DPB_ROWS(128, 4)
-        DPB_ROWS(256, 4)
-        DPB_ROWS(512, 4)
-        DPB_ROWS(1024, 4)
-        DPB_ROWS(1024, 8)
+        DPB_BACK(128, 4, true, 1, 3, true, 1024)
+        DPB_BACK(4096, 4, false, 1, 2, true, 1024)
     }
     else {
-        DPB_ROWS(32, 1)
-        DPB_ROWS(128, 1)
-        DPB_ROWS(256, 1)
-        DPB_ROWS(512, 1)
-        DPB_ROWS(1024, 1)
-        DPB_ROWS(1024, 2)
+        DPB_BACK(32, 1, true, 2, 2, false, 1024)
+        if constexpr (!is_half_v<T>) {
+            DPB_BACK(1024, 2, false, 2, 1, true, 512)
+        }
+        else if constexpr (SHIFT) {
+            DPB_BACK(1280, 2, false, 1, 2, true, 640)
+        }
+        else {
+            DPB_BACK(1024, 2, false, 2, 2, false, 512)
+        }
+        if constexpr (SHIFT) {
+            DPB_BACK(2048, 2, false, 1, 2, false, 1024)
+        }
+        else {
+            DPB_BACK(2048, 4, false, 1, 2, false, 512)
+        }
     }
-#undef DPB_ROWS
+#undef DPB_BACK
     return false;
 }
 
@@ -614,11 +677,16 @@ template <class T, class W> static int run_backward(const NormGradArgs &a, cudaS
     const W *w = a.w ? static_cast<const W *>(a.w->data) : nullptr;
     constexpr int wide = vec_width<T>();
     if (a.rows > 0) {
-        const bool vectors = row_vector(x, a.xm, a.n, sizeof(T), wide) == wide &&
+        const bool aligned = row_vector(x, a.xm, a.n, sizeof(T), wide) == wide &&
                              row_vector(dy, a.dym, a.n, sizeof(T), wide) == wide &&
-                             row_vector(a.dx->data, a.dxm, a.n, sizeof(T), wide) == wide && wide_ok(w, wide, sizeof(W));
+                             row_vector(a.dx->data, a.dxm, a.n, sizeof(T), wide) == wide;
+        // shifted columns: rows one stride apart that start at the same misalignment in dy and x
+        const bool shifted = (a.rows == 1 || (a.xm.outer == 0 && a.dym.outer == 0 && (a.xm.inner - a.dym.inner) % wide == 0)) &&
+                             (reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(dy)) % 16 == 0;
         int st = DPB_OK;
-        if (vectors ? run_rows_backward<T, W, wide>(a, s, st) : run_rows_backward<T, W, 1>(a, s, st)) return st;
+        if (aligned ? run_rows_backward<T, W, wide, false>(a, s, st)
+                    : shifted ? run_rows_backward<T, W, wide, true>(a, s, st) : run_rows_backward<T, W, 1, false>(a, s, st))
+            return st;
     }
     if (a.dw) {
         // before dx, which may overwrite dy or x
