@@ -5,11 +5,11 @@
 //
 // The gradient is a sum of rows by key.  It is taken over the tokens sorted by id, so that every row
 // of the table is written exactly once, by one owner, in an order that does not depend on timing:
-//   1. a stable radix sort of (id, position);
-//   2. the first sorted index of every id (binary search);
-//   3. runs of one id that cross a multiple of kChunk sorted tokens are summed per chunk, so that a
-//      frequent id does not wait for one block;
-//   4. every table row is the sum of its tokens' rows, of its chunks' sums, or zero.
+//   1. a stable radix sort of (id, position), which also marks the ids that occur;
+//   2. one launch that sums the runs of equal ids, kChunk sorted tokens a block (whole runs go to the table,
+//      the parts of runs that cross a chunk's border to a workspace, so that a frequent id does not wait for
+//      one block), and writes zeros to the rows that do not occur;
+//   3. the sums of the parts, in order.
 // Sums are float (double for float64 data), in ascending order of the positions within a chunk and of
 // the chunks; the scale multiplies the finished sum, and the result is rounded once.
 #include "row_ops.cuh"
@@ -17,30 +17,76 @@
 namespace dpb {
 
 constexpr int kThreads = 256;
+constexpr int kAccesses = 4;   // of a thread, kThreads apart: in flight together
+
+// The accesses of all rows in one sequence: access e of a matrix with `per_row` accesses a row.  A block
+// takes kThreads * kAccesses consecutive ones, so that narrow rows share a block and wide ones are split.
+struct RowSequence {
+    FastDiv32 per_row;
+    DPB_D void start(int64_t first, int64_t &row, uint32_t &rest) const
+    {
+        if (first < (int64_t(1) << 31)) {
+            uint32_t q;
+            per_row.divmod(static_cast<uint32_t>(first), q, rest);
+            row = q;
+        }
+        else {
+            row = first / per_row.d;
+            rest = static_cast<uint32_t>(first - row * per_row.d);
+        }
+    }
+};
 
 // ----------------------------------------------------------------------------------------- forward
-template <class T, class I>
+// A copy with a gather: bound by memory, so four accesses of VEC elements in flight a thread.
+template <class T, class I, int VEC>
 __global__ void __launch_bounds__(kThreads) embedding_kernel(const T *table, int64_t ld, const I *ids, acc_t<T> scale, T *out,
-                                                             RowMap om, int64_t vocab, int64_t n)
+                                                             RowMap om, int64_t vocab, int64_t tokens, RowSequence seq)
 {
     using A = acc_t<T>;
-    const uint32_t r = blockIdx.x;
-    const int64_t id = static_cast<int64_t>(ids[r]);
-    T *o = out + om(r);
-    const bool known = id >= 0 && id < vocab;
-    const T *row = table + (known ? id * ld : 0);
-    for (int64_t c = threadIdx.x; c < n; c += kThreads)
-        o[c] = known ? from_acc<T>(to_acc<A>(row[c]) * scale) : from_acc<T>(A(0));
+    using V = vec_t<T, VEC>;
+    cudaGridDependencySynchronize();
+    int64_t row;
+    uint32_t rest;
+    seq.start(int64_t(blockIdx.x) * (kThreads * kAccesses), row, rest);
+    int64_t token[kAccesses], id[kAccesses];
+    uint32_t c[kAccesses];
+#pragma unroll
+    for (int k = 0; k < kAccesses; ++k) {
+        uint32_t q;
+        seq.per_row.divmod(rest + k * kThreads + threadIdx.x, q, c[k]);
+        token[k] = row + q;
+        id[k] = token[k] < tokens ? static_cast<int64_t>(ids[token[k]]) : -1;
+    }
+    V v[kAccesses];
+#pragma unroll
+    for (int k = 0; k < kAccesses; ++k)
+        if (id[k] >= 0 && id[k] < vocab) v[k] = load_vec<V>(table + id[k] * ld + int64_t(c[k]) * VEC);
+#pragma unroll
+    for (int k = 0; k < kAccesses; ++k) {
+        if (token[k] >= tokens) continue;
+        Values<A, VEC> u;
+        u.fill(0);
+        if (id[k] >= 0 && id[k] < vocab) {
+            unpack<A, VEC, T>(v[k], u);
+            u.mul(scale);
+        }
+        *reinterpret_cast<V *>(out + om(static_cast<uint32_t>(token[k])) + int64_t(c[k]) * VEC) = repack<T, VEC, A>(u);
+    }
 }
 
 // ---------------------------------------------------------------------------------- sort of the ids
 // Least significant digit first, `bits` of at most 9 bits a pass; the key of an id outside the table
 // is `vocab`, which sorts behind all rows.  A tile of kTile tokens belongs to one block, a contiguous
 // part of it to each warp, so that ranks within a digit follow the positions (a stable sort).
-constexpr int kTile = 4096;
+// hist[tile][digit] holds the tiles' counts; every placing block forms its own first places from them (up
+// to kJoinedTiles tiles: one launch a pass, the next pass's counts by integer atomics on the way, whose
+// order does not matter), or a scan kernel does that for all.
+constexpr int kTile = 2048;
 constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 512;
+constexpr int kJoinedTiles = 64;
 
 struct SortIn {
     const void *ids;      // of type I in the first pass
@@ -48,201 +94,363 @@ struct SortIn {
     const uint32_t *pos;
 };
 
-template <class I> DPB_D void sort_item(const SortIn &in, bool first, int64_t i, int64_t vocab, uint32_t &key, uint32_t &pos)
+constexpr int kRounds = kTile / kSortThreads;   // items a thread, 32 apart in its warp's part of the tile
+
+struct SortItems {
+    uint32_t key[kRounds], pos[kRounds];
+    uint32_t valid;   // bit k: item k exists
+};
+
+// All items of a thread at once: the loads do not wait for one another.
+template <class I> DPB_D void load_items(const SortIn &in, bool first, int64_t n, int64_t vocab, SortItems &it)
 {
-    if (first) {
-        const int64_t id = static_cast<int64_t>(static_cast<const I *>(in.ids)[i]);
-        key = static_cast<uint32_t>(id >= 0 && id < vocab ? id : vocab);
-        pos = static_cast<uint32_t>(i);
-    }
-    else {
-        key = in.key[i];
-        pos = in.pos[i];
+    const int64_t begin = int64_t(blockIdx.x) * kTile + (threadIdx.x >> 5) * (kTile / kSortWarps) + (threadIdx.x & 31);
+    it.valid = 0;
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+        const int64_t i = begin + k * 32;
+        it.key[k] = it.pos[k] = 0;
+        if (i >= n) continue;
+        it.valid |= 1u << k;
+        if (first) {
+            const int64_t id = static_cast<int64_t>(static_cast<const I *>(in.ids)[i]);
+            it.key[k] = static_cast<uint32_t>(id >= 0 && id < vocab ? id : vocab);
+            it.pos[k] = static_cast<uint32_t>(i);
+        }
+        else {
+            it.key[k] = in.key[i];
+            it.pos[k] = in.pos[i];
+        }
     }
 }
 
 // Counts of a warp's part of the tile per digit.  Lanes with the same digit elect their lowest lane.
-template <class I>
-DPB_D void warp_count(const SortIn &in, bool first, int64_t begin, int64_t end, int64_t vocab, int shift, uint32_t mask,
-                      uint32_t *count)
+DPB_D void warp_count(const SortItems &it, int shift, uint32_t mask, uint32_t *count)
 {
     const int lane = threadIdx.x & 31;
-    for (int64_t at = begin; at < end; at += 32) {
-        const int64_t i = at + lane;
-        uint32_t key = 0, pos, digit = ~0u;
-        if (i < end) {
-            sort_item<I>(in, first, i, vocab, key, pos);
-            digit = (key >> shift) & mask;
-        }
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+        const bool valid = it.valid >> k & 1;
+        const uint32_t digit = valid ? (it.key[k] >> shift) & mask : ~0u;
         const unsigned same = __match_any_sync(0xffffffffu, digit);
-        if (i < end && lane == __ffs(same) - 1) count[digit] += __popc(same);
+        if (valid && lane == __ffs(same) - 1) count[digit] += __popc(same);
         __syncwarp();
     }
 }
 
-// hist[digit][tile]
+// Calls put(k, place) for the items in order: places of a digit from count[digit] on, which advances.
+template <class F> DPB_D void warp_place(const SortItems &it, int shift, uint32_t mask, uint32_t *count, F put)
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+        const bool valid = it.valid >> k & 1;
+        const uint32_t digit = valid ? (it.key[k] >> shift) & mask : ~0u;
+        const unsigned same = __match_any_sync(0xffffffffu, digit);
+        if (valid) put(k, count[digit] + __popc(same & ((1u << lane) - 1)));
+        __syncwarp();
+        if (valid && lane == __ffs(same) - 1) count[digit] += __popc(same);
+        __syncwarp();
+    }
+}
+
+DPB_D void clear_counts(uint32_t (&count)[kSortWarps][kMaxDigits])
+{
+    for (int d = threadIdx.x; d < kSortWarps * kMaxDigits; d += kSortThreads) (&count[0][0])[d] = 0;
+}
+
+// Counts of one digit; `later` counters behind them (of the later passes' tiles) are set to zero, and the marks
+// of the ids too (`marks` of 4 ids, or none).
 template <class I>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortIn in, bool first, int64_t n, int64_t vocab, int shift,
-                                                                  int bits, uint32_t *hist)
+                                                                  int bits, uint32_t *hist, int later, uint32_t *mark, int64_t marks)
 {
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
-    const int digits = 1 << bits, warp = threadIdx.x >> 5;
-    for (int d = threadIdx.x; d < kSortWarps * kMaxDigits; d += kSortThreads) (&count[0][0])[d] = 0;
+    cudaGridDependencySynchronize();
+    SortItems it;
+    load_items<I>(in, first, n, vocab, it);
+    const int digits = 1 << bits;
+    clear_counts(count);
+    for (int d = threadIdx.x; d < later * digits; d += kSortThreads)
+        hist[(int64_t(1 + d / digits) * gridDim.x + blockIdx.x) * digits + d % digits] = 0;
+    for (int64_t i = int64_t(blockIdx.x) * kSortThreads + threadIdx.x; i < marks; i += int64_t(gridDim.x) * kSortThreads) mark[i] = 0;
     __syncthreads();
-    constexpr int part = kTile / kSortWarps;
-    const int64_t begin = min(n, int64_t(blockIdx.x) * kTile + int64_t(warp) * part), end = min(n, begin + part);
-    warp_count<I>(in, first, begin, end, vocab, shift, digits - 1, count[warp]);
+    warp_count(it, shift, digits - 1, count[threadIdx.x >> 5]);
     __syncthreads();
     for (int d = threadIdx.x; d < digits; d += kSortThreads) {
         uint32_t s = 0;
         for (int w = 0; w < kSortWarps; ++w) s += count[w][d];
-        hist[int64_t(d) * gridDim.x + blockIdx.x] = s;
+        hist[int64_t(blockIdx.x) * digits + d] = s;
     }
 }
 
-// Exclusive scan of `n` counters in place by one block.
-__global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t *hist, int64_t n)
+// First place of every (tile, digit) in place of its count, by one block: the digits' totals are scanned,
+// then each digit runs through its tiles.
+__global__ void __launch_bounds__(kMaxDigits) sort_scan_kernel(uint32_t *hist, int64_t tiles, int digits)
 {
-    __shared__ uint32_t warp_sum[32];
-    __shared__ uint32_t carry_s;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) carry_s = 0;
+    __shared__ uint32_t total[kMaxDigits];
+    cudaGridDependencySynchronize();
+    const int d = threadIdx.x;
+    uint32_t s = 0;
+    if (d < digits)
+        for (int64_t t = 0; t < tiles; ++t) s += hist[t * digits + d];
+    total[d] = s;
     __syncthreads();
-    for (int64_t base = 0; base < n; base += 1024) {
-        const int64_t i = base + threadIdx.x;
-        const uint32_t v = i < n ? hist[i] : 0;
-        uint32_t s = v;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t t = __shfl_up_sync(0xffffffffu, s, d);
-            if (lane >= d) s += t;
+    if (d == 0) {
+        uint32_t at = 0;
+        for (int k = 0; k < digits; ++k) {
+            const uint32_t c = total[k];
+            total[k] = at;
+            at += c;
         }
-        if (lane == 31) warp_sum[warp] = s;
-        __syncthreads();
-        if (warp == 0) {
-            uint32_t t = warp_sum[lane];
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t u = __shfl_up_sync(0xffffffffu, t, d);
-                if (lane >= d) t += u;
-            }
-            warp_sum[lane] = t;
-        }
-        __syncthreads();
-        const uint32_t before = carry_s + (warp > 0 ? warp_sum[warp - 1] : 0);
-        if (i < n) hist[i] = before + s - v;
-        __syncthreads();
-        if (threadIdx.x == 0) carry_s += warp_sum[31];
-        __syncthreads();
+    }
+    __syncthreads();
+    if (d >= digits) return;
+    uint32_t at = total[d];
+    for (int64_t t = 0; t < tiles; ++t) {
+        const uint32_t c = hist[t * digits + d];
+        hist[t * digits + d] = at;
+        at += c;
     }
 }
 
-// Moves every (key, position) to its place: first place of its digit and tile (from the scan), plus the
-// earlier warps' counts of the digit, plus its rank in its own warp's part.
-template <class I>
+// Exclusive scan of kMaxDigits counters in shared memory by kSortThreads threads, two counters each.
+DPB_D void scan_digits(uint32_t *v, uint32_t *warp_sum)
+{
+    static_assert(kMaxDigits == 2 * kSortThreads, "two counters a thread");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t a = v[2 * threadIdx.x], b = v[2 * threadIdx.x + 1];
+    uint32_t s = a + b;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, s, d);
+        if (lane >= d) s += t;
+    }
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    uint32_t before = s - a - b;
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    v[2 * threadIdx.x] = before;
+    v[2 * threadIdx.x + 1] = before + a;
+    __syncthreads();
+}
+
+// Turns the warps' counts of each digit into the warps' first places, from the digit's first place on.
+DPB_D void warp_places(uint32_t (&count)[kSortWarps][kMaxDigits], int d, uint32_t from)
+{
+    for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = count[w][d];
+        count[w][d] = from;
+        from += c;
+    }
+}
+
+// Moves every (key, position) to its place: first place of its digit and tile, plus the earlier warps' counts
+// of the digit, plus its rank in its own warp's part.  JOINED: `hist` holds counts; `next` (or null) gathers
+// the counts of the next digit in the tiles that the items move to.  The last pass (mark not null) marks the ids.
+template <class I, bool JOINED>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortIn in, bool first, int64_t n, int64_t vocab, int shift,
-                                                                  int bits, const uint32_t *hist, uint32_t *key_out,
-                                                                  uint32_t *pos_out)
+                                                                  int bits, const uint32_t *hist, uint32_t *next,
+                                                                  uint32_t *key_out, uint32_t *pos_out, uint8_t *mark)
 {
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
-    const int digits = 1 << bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int d = threadIdx.x; d < kSortWarps * kMaxDigits; d += kSortThreads) (&count[0][0])[d] = 0;
-    __syncthreads();
-    constexpr int part = kTile / kSortWarps;
-    const int64_t begin = min(n, int64_t(blockIdx.x) * kTile + int64_t(warp) * part), end = min(n, begin + part);
-    const uint32_t mask = digits - 1;
-    warp_count<I>(in, first, begin, end, vocab, shift, mask, count[warp]);
-    __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += kSortThreads) {
-        uint32_t s = hist[int64_t(d) * gridDim.x + blockIdx.x];
-        for (int w = 0; w < kSortWarps; ++w) {
-            const uint32_t c = count[w][d];
-            count[w][d] = s;
-            s += c;
+    __shared__ uint32_t place[kMaxDigits], warp_sum[kSortWarps];
+    cudaGridDependencySynchronize();
+    SortItems it;
+    load_items<I>(in, first, n, vocab, it);
+    const int digits = 1 << bits, d0 = 2 * threadIdx.x;
+    clear_counts(count);
+    uint2 earlier = {0, 0}, all = {0, 0};   // this thread's two digits: in the tiles before, in all tiles
+    if (d0 < digits) {
+        const uint2 *h = reinterpret_cast<const uint2 *>(hist + d0);
+        if constexpr (JOINED) {
+#pragma unroll 16
+            for (int t = 0; t < static_cast<int>(gridDim.x); ++t) {
+                const uint2 c = h[t * digits / 2];
+                if (t < static_cast<int>(blockIdx.x)) {
+                    earlier.x += c.x;
+                    earlier.y += c.y;
+                }
+                all.x += c.x;
+                all.y += c.y;
+            }
         }
+        else earlier = h[int64_t(blockIdx.x) * digits / 2];
+    }
+    place[d0] = all.x;
+    place[d0 + 1] = all.y;
+    __syncthreads();
+    if constexpr (JOINED) scan_digits(place, warp_sum);
+    const uint32_t mask = digits - 1;
+    uint32_t *mine = count[threadIdx.x >> 5];
+    warp_count(it, shift, mask, mine);
+    __syncthreads();
+    if (d0 < digits) {
+        warp_places(count, d0, place[d0] + earlier.x);
+        warp_places(count, d0 + 1, place[d0 + 1] + earlier.y);
     }
     __syncthreads();
-    for (int64_t at = begin; at < end; at += 32) {
-        const int64_t i = at + lane;
-        uint32_t key = 0, pos = 0, digit = ~0u;
-        if (i < end) {
-            sort_item<I>(in, first, i, vocab, key, pos);
-            digit = (key >> shift) & mask;
+    warp_place(it, shift, mask, mine, [&](int k, uint32_t to) {
+        key_out[to] = it.key[k];
+        pos_out[to] = it.pos[k];
+        if (JOINED && next) atomicAdd(next + (to / kTile) * digits + ((it.key[k] >> (shift + bits)) & mask), 1u);
+        if (mark && it.key[k] < vocab) mark[it.key[k]] = 1;
+    });
+}
+
+// All passes of up to kTile tokens by one block, through shared memory.
+template <class I>
+__global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const I *ids, int64_t n, int64_t vocab, int passes, int bits,
+                                                                 uint32_t *key_out, uint32_t *pos_out, uint8_t *mark, int64_t marks)
+{
+    __shared__ uint32_t count[kSortWarps][kMaxDigits];
+    __shared__ uint32_t place[kMaxDigits], warp_sum[kSortWarps], keys[kTile], positions[kTile];
+    cudaGridDependencySynchronize();
+    SortItems it;
+    load_items<I>({ids, nullptr, nullptr}, true, n, vocab, it);
+    for (int64_t i = threadIdx.x; i < marks; i += kSortThreads) reinterpret_cast<uint32_t *>(mark)[i] = 0;
+    const int d0 = 2 * threadIdx.x;
+    const uint32_t mask = (1u << bits) - 1;
+    uint32_t *mine = count[threadIdx.x >> 5];
+    for (int p = 0; p < passes; ++p) {
+        if (p > 0) {
+            const int begin = (threadIdx.x >> 5) * (kTile / kSortWarps) + (threadIdx.x & 31);
+#pragma unroll
+            for (int k = 0; k < kRounds; ++k) {
+                if (!(it.valid >> k & 1)) continue;
+                it.key[k] = keys[begin + k * 32];
+                it.pos[k] = positions[begin + k * 32];
+            }
         }
-        const unsigned same = __match_any_sync(0xffffffffu, digit);
-        if (i < end) {
-            const uint32_t to = count[warp][digit] + __popc(same & ((1u << lane) - 1));
-            key_out[to] = key;
-            pos_out[to] = pos;
+        clear_counts(count);
+        __syncthreads();
+        warp_count(it, p * bits, mask, mine);
+        __syncthreads();
+        for (int d = d0; d < d0 + 2; ++d) {
+            uint32_t c = 0;
+            for (int w = 0; w < kSortWarps; ++w) c += count[w][d];
+            place[d] = c;
         }
-        __syncwarp();
-        if (i < end && lane == __ffs(same) - 1) count[warp][digit] += __popc(same);
-        __syncwarp();
+        __syncthreads();
+        scan_digits(place, warp_sum);
+        warp_places(count, d0, place[d0]);
+        warp_places(count, d0 + 1, place[d0 + 1]);
+        __syncthreads();
+        const bool last = p == passes - 1;
+        warp_place(it, p * bits, mask, mine, [&](int k, uint32_t to) {
+            (last ? key_out : keys)[to] = it.key[k];
+            (last ? pos_out : positions)[to] = it.pos[k];
+            if (last && it.key[k] < vocab) mark[it.key[k]] = 1;
+        });
+        __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------------------------------- gradient
-constexpr int kChunk = 128;
+constexpr int kChunk = 32;      // sorted tokens of a block
+constexpr int kInFlight = 8;    // rows' loads of a thread in flight
 
-// first[v] = number of sorted keys below v, for v = 0 .. vocab
-__global__ void __launch_bounds__(kThreads) segment_start_kernel(const uint32_t *key, int64_t n, int64_t vocab, uint32_t *first)
-{
-    const int64_t v = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-    if (v > vocab) return;
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (key[mid] < static_cast<uint32_t>(v)) lo = mid + 1;
-        else hi = mid;
-    }
-    first[v] = static_cast<uint32_t>(lo);
-}
-
-// Sums of the runs that cross a chunk's borders: part[2 k] for a run that came in from chunk k - 1,
-// part[2 k + 1] for one that starts in chunk k and goes on in chunk k + 1.
-template <class T>
-__global__ void __launch_bounds__(kThreads) embedding_chunk_kernel(const T *dout, RowMap dm, const uint32_t *key,
-                                                                   const uint32_t *pos, const uint32_t *first,
-                                                                   int64_t n_tokens, int64_t vocab, int64_t n, acc_t<T> *part)
+// The first blocks sum runs: block (chunk k, column tile) walks its tokens in order.  A run that lies in the chunk goes
+// to the table; part[2 k] takes the sum of one that came in from chunk k - 1 (and may go on), part[2 k + 1]
+// of one that starts here and goes on.  The other blocks write the rows that do not occur, kAccesses
+// accesses a thread: reads and writes of the two kinds overlap.
+template <class T, class O, int VEC>
+__global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout, RowMap dm, const uint32_t *key, const uint32_t *pos,
+                                                                  uint32_t tokens, const uint8_t *mark, acc_t<T> *part,
+                                                                  acc_t<T> scale, O *dtable, int64_t ld, uint32_t vocab,
+                                                                  RowSequence seq, uint32_t sum_blocks, FastDiv32 tiles)
 {
     using A = acc_t<T>;
-    const int64_t k = blockIdx.x, begin = k * kChunk, end = min(n_tokens, begin + kChunk);
-    for (int side = 0; side < 2; ++side) {
-        const uint32_t id = key[side == 0 ? begin : end - 1];
-        if (id >= vocab) continue;
-        const int64_t from = first[id], to = first[id + 1];
-        if (side == 0 ? from >= begin : (to <= end || from < begin)) continue;
-        const int64_t b = max(begin, from), e = min(end, to);
-        for (int64_t c = int64_t(blockIdx.y) * kThreads + threadIdx.x; c < n; c += int64_t(gridDim.y) * kThreads) {
-            A s = 0;
-            for (int64_t i = b; i < e; ++i) s += to_acc<A>(dout[dm(pos[i]) + c]);
-            part[(2 * k + side) * n + c] = s;
+    using V = vec_t<T, VEC>;
+    using VO = vec_t<O, VEC>;
+    using Vals = Values<A, VEC>;
+    cudaGridDependencySynchronize();
+    if (blockIdx.x >= sum_blocks) {
+        int64_t row;
+        uint32_t rest;
+        seq.start(int64_t(blockIdx.x - sum_blocks) * (kThreads * kAccesses), row, rest);
+        Vals zero;
+        zero.fill(0);
+        const VO z = repack<O, VEC, A>(zero);
+#pragma unroll
+        for (int k = 0; k < kAccesses; ++k) {
+            uint32_t q, c;
+            seq.per_row.divmod(rest + k * kThreads + threadIdx.x, q, c);
+            const int64_t v = row + q;
+            if (v < vocab && !mark[v]) *reinterpret_cast<VO *>(dtable + v * ld + int64_t(c) * VEC) = z;
         }
+        return;
     }
-}
-
-template <class T, class O>
-__global__ void __launch_bounds__(kThreads) embedding_rows_kernel(const T *dout, RowMap dm, const uint32_t *pos,
-                                                                  const uint32_t *first, const acc_t<T> *part, acc_t<T> scale,
-                                                                  int64_t n, O *dtable, int64_t ld)
-{
-    using A = acc_t<T>;
-    const int64_t v = blockIdx.x;
-    const int64_t from = first[v], to = first[v + 1];
-    O *o = dtable + v * ld;
-    const int64_t k0 = from / kChunk, k1 = (to - 1) / kChunk;
-    for (int64_t c = threadIdx.x; c < n; c += kThreads) {
-        A s = 0;
-        if (to > from) {
-            if (k0 == k1)
-                for (int64_t i = from; i < to; ++i) s += to_acc<A>(dout[dm(pos[i]) + c]);
-            else {
-                s = part[(2 * k0 + 1) * n + c];
-                for (int64_t k = k0 + 1; k <= k1; ++k) s += part[2 * k * n + c];
+    __shared__ uint32_t keys[kChunk + 2];   // with the token before and the token behind the chunk
+    __shared__ int64_t rows[kChunk];
+    uint32_t k, tile;
+    tiles.divmod(blockIdx.x, k, tile);
+    const uint32_t begin = k * kChunk, count = min(tokens - begin, uint32_t(kChunk));
+    if (threadIdx.x < count + 2) {
+        const int64_t i = int64_t(begin) + threadIdx.x - 1;
+        keys[threadIdx.x] = i >= 0 && i < tokens ? key[i] : ~0u;
+    }
+    if (threadIdx.x < count) rows[threadIdx.x] = dm(pos[begin + threadIdx.x]);
+    __syncthreads();
+    const int64_t c = int64_t(tile) * kThreads + threadIdx.x;
+    if (c >= seq.per_row.d) return;
+    Vals s, u;
+    s.fill(0);
+    bool whole = keys[0] != keys[1];   // the current run starts in this chunk
+    for (uint32_t i0 = 0; i0 < count; i0 += kInFlight) {
+        V v[kInFlight];
+#pragma unroll
+        for (int j = 0; j < kInFlight; ++j)
+            if (i0 + j < count && keys[i0 + j + 1] < vocab) v[j] = load_vec<V>(dout + rows[i0 + j] + c * VEC);
+#pragma unroll
+        for (int j = 0; j < kInFlight; ++j) {
+            const uint32_t i = i0 + j;
+            if (i >= count) break;
+            const uint32_t id = keys[i + 1];
+            if (id >= vocab) return;   // behind all rows of the table
+            unpack<A, VEC, T>(v[j], u);
+            s.add(u);
+            const bool ends = keys[i + 2] != id;
+            if (!ends && i + 1 < count) continue;
+            if (whole && ends) {
+                s.mul(scale);
+                *reinterpret_cast<VO *>(dtable + id * ld + c * VEC) = repack<O, VEC, A>(s);
             }
+            else *reinterpret_cast<Vals *>(part + (int64_t(2 * k + whole) * seq.per_row.d + c) * VEC) = s;
+            s.fill(0);
+            whole = true;
         }
-        o[c] = from_acc<O>(s * scale);
     }
+}
+
+// Runs over several chunks: the block of the chunk in which one ends adds its parts in order.
+template <class A, class O, int VEC>
+__global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t *key, uint32_t tokens, const A *part, A scale,
+                                                                  O *dtable, int64_t ld, uint32_t vocab, uint32_t per_row)
+{
+    using Vals = Values<A, VEC>;
+    cudaGridDependencySynchronize();
+    const uint32_t k = blockIdx.x + 1, begin = k * kChunk, end = min(tokens, begin + kChunk);
+    const uint32_t id = key[begin];
+    // a run that came in and ends here
+    if (id >= vocab || key[begin - 1] != id || (end < tokens && key[end - 1] == id && key[end] == id)) return;
+    const uint32_t c = blockIdx.y * kThreads + threadIdx.x;
+    // chunks before this one whose last token belongs to the run, a warp at a time
+    uint32_t first = k;   // the first chunk that the run came into
+    for (;;) {
+        const int64_t at = int64_t(first) - 1 - (threadIdx.x & 31);   // chunk `at` passes the run on to at + 1
+        const unsigned on = __ballot_sync(0xffffffffu, at >= 1 && key[at * kChunk - 1] == id);
+        const int run = on == 0xffffffffu ? 32 : __ffs(~on) - 1;
+        first -= run;
+        if (run < 32) break;
+    }
+    if (c >= per_row) return;
+    const Vals *p = reinterpret_cast<const Vals *>(part) + c;
+    Vals s = p[int64_t(2 * (first - 1) + 1) * per_row];
+#pragma unroll 8
+    for (uint32_t g = first; g <= k; ++g) s.add(p[int64_t(2 * g) * per_row]);
+    s.mul(scale);
+    *reinterpret_cast<vec_t<O, VEC> *>(dtable + id * ld + int64_t(c) * VEC) = repack<O, VEC, A>(s);
 }
 
 // --------------------------------------------------------------------------------------- launchers
@@ -253,36 +461,81 @@ struct EmbedArgs {
     double scale;
 };
 
+static unsigned sequence_blocks(int64_t rows, int64_t per_row)
+{
+    return static_cast<unsigned>(ceil_div(rows * per_row, kThreads * kAccesses));
+}
+
+template <class T, class I, int VEC> static void launch_forward(const EmbedArgs &a, cudaStream_t s)
+{
+    const int64_t per_row = a.n / VEC;
+    launch_after_previous(embedding_kernel<T, I, VEC>, sequence_blocks(a.tokens, per_row), unsigned(kThreads), s,
+                          static_cast<const T *>(a.table->data), a.ld, static_cast<const I *>(a.ids->data), acc_t<T>(a.scale),
+                          static_cast<T *>(a.out->data), a.om, a.vocab, a.tokens, RowSequence{FastDiv32(uint32_t(per_row))});
+}
+
+// Accesses of 16 bytes where all rows allow them, else (float16) of 4 bytes, else single elements.
 template <class T, class I> static int run_forward(const EmbedArgs &a, cudaStream_t s)
 {
-    embedding_kernel<T, I><<<static_cast<unsigned>(a.tokens), kThreads, 0, s>>>(
-        static_cast<const T *>(a.table->data), a.ld, static_cast<const I *>(a.ids->data), acc_t<T>(a.scale),
-        static_cast<T *>(a.out->data), a.om, a.vocab, a.n);
+    constexpr int wide = vec_width<T>();
+    const RowMap table = {0, a.ld, FastDiv32(1)};
+    const int v = std::min(row_vector(a.out->data, a.om, a.n, sizeof(T), wide), row_vector(a.table->data, table, a.n, sizeof(T), wide));
+    if (v == wide) launch_forward<T, I, wide>(a, s);
+    else if (is_half_v<T> && v >= 2) launch_forward<T, I, is_half_v<T> ? 2 : 1>(a, s);
+    else launch_forward<T, I, 1>(a, s);
     note_kernel("embedding");
     return check_launch("embedding");
 }
 
-// Sorted keys and positions of the ids in `work` (4 arrays of `n`, then the counters).
-template <class I> static void sort_ids(const void *ids, int64_t n, int64_t vocab, uint32_t *work, uint32_t *&key, uint32_t *&pos,
-                                        cudaStream_t s)
+static int64_t sort_words(int64_t n)   // of the sort's workspace
+{
+    return 4 * n + 4 * ceil_div(n, kTile) * kMaxDigits;
+}
+
+// Sorted keys and positions of the ids in `work` (two pairs of arrays of `n`, then the counters of the passes), and
+// marks of the ids that occur.
+template <class I> static void sort_ids(const void *ids, int64_t n, int64_t vocab, uint32_t *work, uint8_t *mark, uint32_t *&key,
+                                        uint32_t *&pos, cudaStream_t s)
 {
     int bits = 1;
     while ((int64_t(1) << bits) <= vocab) ++bits;
     const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes;
-    const int64_t tiles = ceil_div(n, kTile);
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(n, kTile)), counters = tiles << width, marks = ceil_div(vocab, 4);
+    const unsigned grid = static_cast<unsigned>(tiles), block = kSortThreads;
+    if (tiles == 1) {
+        key = work;
+        pos = work + n;
+        launch_after_previous(sort_tile_kernel<I>, grid, block, s, static_cast<const I *>(ids), n, vocab, passes, width, key, pos, mark,
+                              marks);
+        note_kernel("sort_tile");
+        return;
+    }
+    const bool joined = tiles <= kJoinedTiles;
     uint32_t *bufs[2][2] = {{work, work + n}, {work + 2 * n, work + 3 * n}};
     uint32_t *hist = work + 4 * n;
     SortIn in = {ids, nullptr, nullptr};
     for (int p = 0; p < passes; ++p) {
         const int shift = p * width;
-        const unsigned grid = static_cast<unsigned>(tiles);
-        sort_count_kernel<I><<<grid, kSortThreads, 0, s>>>(in, p == 0, n, vocab, shift, width, hist);
-        note_kernel("sort_count");
-        sort_scan_kernel<<<1, 1024, 0, s>>>(hist, tiles << width);
-        note_kernel("sort_scan");
         key = bufs[p & 1][0];
         pos = bufs[p & 1][1];
-        sort_place_kernel<I><<<grid, kSortThreads, 0, s>>>(in, p == 0, n, vocab, shift, width, hist, key, pos);
+        uint8_t *last = p + 1 == passes ? mark : nullptr;
+        if (!joined || p == 0) {
+            launch_after_previous(sort_count_kernel<I>, grid, block, s, in, p == 0, n, vocab, shift, width, hist, joined ? passes - 1 : 0,
+                                  reinterpret_cast<uint32_t *>(mark), p == 0 ? marks : 0);
+            note_kernel("sort_count");
+        }
+        if (joined) {
+            uint32_t *next = p + 1 < passes ? hist + counters : nullptr;
+            launch_after_previous(sort_place_kernel<I, true>, grid, block, s, in, p == 0, n, vocab, shift, width, hist, next, key, pos,
+                                  last);
+            hist += counters;
+        }
+        else {
+            launch_after_previous(sort_scan_kernel, 1u, unsigned(kMaxDigits), s, hist, tiles, 1 << width);
+            note_kernel("sort_scan");
+            launch_after_previous(sort_place_kernel<I, false>, grid, block, s, in, p == 0, n, vocab, shift, width, hist,
+                                  static_cast<uint32_t *>(nullptr), key, pos, last);
+        }
         note_kernel("sort_place");
         in = {nullptr, key, pos};
     }
@@ -295,32 +548,55 @@ struct EmbedGradArgs {
     double scale;
 };
 
+template <class T, class O, int VEC>
+static void launch_sums(const EmbedGradArgs &a, const uint32_t *key, const uint32_t *pos, const uint8_t *mark, acc_t<T> *part,
+                        cudaStream_t s)
+{
+    using A = acc_t<T>;
+    const int64_t per_row = a.n / VEC, tiles = ceil_div(per_row, kThreads), chunks = ceil_div(a.tokens, kChunk);
+    O *dtable = static_cast<O *>(a.dtable->data);
+    launch_after_previous(embedding_sums_kernel<T, O, VEC>, static_cast<unsigned>(chunks * tiles) + sequence_blocks(a.vocab, per_row),
+                          unsigned(kThreads), s, static_cast<const T *>(a.dout->data), a.dm, key, pos, uint32_t(a.tokens), mark, part,
+                          A(a.scale), dtable, a.ld, uint32_t(a.vocab), RowSequence{FastDiv32(uint32_t(per_row))},
+                          uint32_t(chunks * tiles), FastDiv32(uint32_t(tiles)));
+    note_kernel("embedding_sums");
+    if (chunks < 2) return;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(chunks - 1), static_cast<unsigned>(tiles));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    if (tuning_pdl()) {
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    cudaLaunchKernelEx(&cfg, embedding_join_kernel<A, O, VEC>, key, uint32_t(a.tokens), static_cast<const A *>(part), A(a.scale), dtable,
+                       a.ld, uint32_t(a.vocab), uint32_t(per_row));
+    note_kernel("embedding_join");
+}
+
 template <class T, class O> static int run_backward(const EmbedGradArgs &a, cudaStream_t s)
 {
     using A = acc_t<T>;
-    const int64_t tiles = ceil_div(a.tokens, kTile), chunks = ceil_div(a.tokens, kChunk);
-    const size_t words = static_cast<size_t>(4 * a.tokens + tiles * kMaxDigits + a.vocab + 1);
-    const size_t head = (words * 4 + 255) / 256 * 256;
+    const int64_t chunks = ceil_div(a.tokens, kChunk);
+    const size_t words = static_cast<size_t>(sort_words(a.tokens) + ceil_div(a.vocab, 4)) * 4;   // then a mark a row
+    const size_t head = (words + 255) / 256 * 256;
     void *work = nullptr;
     DPB_TRY(dpb_malloc(head + static_cast<size_t>(2 * chunks * a.n) * sizeof(A), s, &work));
     uint32_t *w = static_cast<uint32_t *>(work), *key = nullptr, *pos = nullptr;
-    uint32_t *first = w + 4 * a.tokens + tiles * kMaxDigits;
+    uint8_t *mark = reinterpret_cast<uint8_t *>(w + sort_words(a.tokens));
     A *part = reinterpret_cast<A *>(static_cast<char *>(work) + head);
-    if (a.tokens > 0) {
-        if (a.ids->typenum == DPB_INT32) sort_ids<int32_t>(a.ids->data, a.tokens, a.vocab, w, key, pos, s);
-        else sort_ids<int64_t>(a.ids->data, a.tokens, a.vocab, w, key, pos, s);
-    }
-    segment_start_kernel<<<static_cast<unsigned>(ceil_div(a.vocab + 1, kThreads)), kThreads, 0, s>>>(key, a.tokens, a.vocab, first);
-    note_kernel("segment_start");
-    const T *dout = static_cast<const T *>(a.dout->data);
-    if (a.tokens > kChunk) {
-        const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(std::min<int64_t>(ceil_div(a.n, kThreads), 16)));
-        embedding_chunk_kernel<T><<<grid, kThreads, 0, s>>>(dout, a.dm, key, pos, first, a.tokens, a.vocab, a.n, part);
-        note_kernel("embedding_chunk");
-    }
-    embedding_rows_kernel<T, O><<<static_cast<unsigned>(a.vocab), kThreads, 0, s>>>(
-        dout, a.dm, pos, first, part, A(a.scale), a.n, static_cast<O *>(a.dtable->data), a.ld);
-    note_kernel("embedding_rows");
+    if (a.ids->typenum == DPB_INT32) sort_ids<int32_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, s);
+    else sort_ids<int64_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, s);
+    constexpr int wide = vec_width<T>();
+    int v = a.tokens > 0 ? row_vector(a.dout->data, a.dm, a.n, sizeof(T), wide) : wide;
+    // (a float32 gradient of float16 data is written in accesses of at most 32 bytes)
+    while (v > 1 && (a.n % v || a.ld % v || !is_aligned(a.dtable->data, v * sizeof(O)))) v /= 2;
+    if (v == wide) launch_sums<T, O, wide>(a, key, pos, mark, part, s);
+    else if (is_half_v<T> && v >= 2) launch_sums<T, O, is_half_v<T> ? 2 : 1>(a, key, pos, mark, part, s);
+    else launch_sums<T, O, 1>(a, key, pos, mark, part, s);
     const int st = check_launch("embedding_backward");
     dpb_free(work, s);
     return st;
@@ -334,6 +610,7 @@ static int check_table(const dpb_array &t, int64_t &vocab, int64_t &n, int64_t &
     vocab = t.shape[0];
     n = t.shape[1];
     if (vocab > kMaxRows) return set_error(DPB_ERR_VALUE, "%s: more than 2^31 - 1 rows are not supported", what);
+    if (n > kMaxRows / 2) return set_error(DPB_ERR_VALUE, "%s: rows of more than 2^30 - 1 elements are not supported", what);
     const std::vector<int64_t> st = strides_of(t);
     if (n > 1 && st[1] != 1) return set_error(DPB_ERR_VALUE, "%s: rows of unit stride are needed", what);
     ld = st[0];
