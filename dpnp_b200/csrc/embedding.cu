@@ -6,7 +6,7 @@
 // The gradient is a sum of rows by key.  It is taken over the tokens sorted by id, so that every row
 // of the table is written exactly once, by one owner, in an order that does not depend on timing:
 //   1. a stable radix sort of (id, position), which also marks the ids that occur;
-//   2. one launch that sums the runs of equal ids, kChunk sorted tokens a block (whole runs go to the table,
+//   2. one launch that sums the runs of equal ids, a chunk of 32 to 128 sorted tokens a block (whole runs go to the table,
 //      the parts of runs that cross a chunk's border to a workspace, so that a frequent id does not wait for
 //      one block), and writes zeros to the rows that do not occur;
 //   3. the sums of the parts, in order.
@@ -83,10 +83,38 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const T *table, int
 // to kJoinedTiles tiles: one launch a pass, the next pass's counts by integer atomics on the way, whose
 // order does not matter), or a scan kernel does that for all.
 constexpr int kTile = 2048;
-constexpr int kSortThreads = 256;
+constexpr int kSortThreads = kThreads;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 512;
 constexpr int kJoinedTiles = 64;
+
+// Zeros for a range of a matrix's accesses: the sort occupies few SMs, and its launches carry blocks that
+// begin with the gradient's zeros (of rows that occur, too: they are written again later).
+struct ZeroRows {
+    char *base;
+    int64_t row_bytes;   // from one row to the next
+    int access;          // bytes: 16, 8, 4 or 2
+    RowSequence seq;
+    int64_t rows, first;   // first access of this launch
+    int64_t blocks;
+};
+DPB_D void zero_rows(const ZeroRows &z, int64_t block)
+{
+    int64_t row;
+    uint32_t rest;
+    z.seq.start(z.first + block * (kThreads * kAccesses), row, rest);
+#pragma unroll
+    for (int k = 0; k < kAccesses; ++k) {
+        uint32_t q, c;
+        z.seq.per_row.divmod(rest + k * kThreads + threadIdx.x, q, c);
+        if (row + q >= z.rows) continue;
+        char *p = z.base + (row + q) * z.row_bytes + int64_t(c) * z.access;
+        if (z.access == 16) *reinterpret_cast<int4 *>(p) = make_int4(0, 0, 0, 0);
+        else if (z.access == 8) *reinterpret_cast<int2 *>(p) = make_int2(0, 0);
+        else if (z.access == 4) *reinterpret_cast<int *>(p) = 0;
+        else *reinterpret_cast<short *>(p) = 0;
+    }
+}
 
 struct SortIn {
     const void *ids;      // of type I in the first pass
@@ -163,17 +191,19 @@ DPB_D void clear_counts(uint32_t (&count)[kSortWarps][kMaxDigits])
 // of the ids too (`marks` of 4 ids, or none).
 template <class I>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortIn in, bool first, int64_t n, int64_t vocab, int shift,
-                                                                  int bits, uint32_t *hist, int later, uint32_t *mark, int64_t marks)
+                                                                  int bits, uint32_t *hist, int tiles, int later, uint32_t *mark, int64_t marks,
+                                                                  ZeroRows zero)
 {
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
     cudaGridDependencySynchronize();
+    if (blockIdx.x >= tiles) return zero_rows(zero, blockIdx.x - tiles);
     SortItems it;
     load_items<I>(in, first, n, vocab, it);
     const int digits = 1 << bits;
     clear_counts(count);
     for (int d = threadIdx.x; d < later * digits; d += kSortThreads)
-        hist[(int64_t(1 + d / digits) * gridDim.x + blockIdx.x) * digits + d % digits] = 0;
-    for (int64_t i = int64_t(blockIdx.x) * kSortThreads + threadIdx.x; i < marks; i += int64_t(gridDim.x) * kSortThreads) mark[i] = 0;
+        hist[(int64_t(1 + d / digits) * tiles + blockIdx.x) * digits + d % digits] = 0;
+    for (int64_t i = int64_t(blockIdx.x) * kSortThreads + threadIdx.x; i < marks; i += int64_t(tiles) * kSortThreads) mark[i] = 0;
     __syncthreads();
     warp_count(it, shift, digits - 1, count[threadIdx.x >> 5]);
     __syncthreads();
@@ -251,11 +281,13 @@ DPB_D void warp_places(uint32_t (&count)[kSortWarps][kMaxDigits], int d, uint32_
 template <class I, bool JOINED>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortIn in, bool first, int64_t n, int64_t vocab, int shift,
                                                                   int bits, const uint32_t *hist, uint32_t *next,
-                                                                  uint32_t *key_out, uint32_t *pos_out, uint8_t *mark)
+                                                                  uint32_t *key_out, uint32_t *pos_out, uint8_t *mark, int tiles,
+                                                                  ZeroRows zero)
 {
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
     __shared__ uint32_t place[kMaxDigits], warp_sum[kSortWarps];
     cudaGridDependencySynchronize();
+    if (blockIdx.x >= tiles) return zero_rows(zero, blockIdx.x - tiles);
     SortItems it;
     load_items<I>(in, first, n, vocab, it);
     const int digits = 1 << bits, d0 = 2 * threadIdx.x;
@@ -265,7 +297,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortIn in, boo
         const uint2 *h = reinterpret_cast<const uint2 *>(hist + d0);
         if constexpr (JOINED) {
 #pragma unroll 16
-            for (int t = 0; t < static_cast<int>(gridDim.x); ++t) {
+            for (int t = 0; t < tiles; ++t) {
                 const uint2 c = h[t * digits / 2];
                 if (t < static_cast<int>(blockIdx.x)) {
                     earlier.x += c.x;
@@ -301,11 +333,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortIn in, boo
 // All passes of up to kTile tokens by one block, through shared memory.
 template <class I>
 __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const I *ids, int64_t n, int64_t vocab, int passes, int bits,
-                                                                 uint32_t *key_out, uint32_t *pos_out, uint8_t *mark, int64_t marks)
+                                                                 uint32_t *key_out, uint32_t *pos_out, uint8_t *mark, int64_t marks,
+                                                                 ZeroRows zero)
 {
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
     __shared__ uint32_t place[kMaxDigits], warp_sum[kSortWarps], keys[kTile], positions[kTile];
     cudaGridDependencySynchronize();
+    if (blockIdx.x >= 1) return zero_rows(zero, blockIdx.x - 1);
     SortItems it;
     load_items<I>({ids, nullptr, nullptr}, true, n, vocab, it);
     for (int64_t i = threadIdx.x; i < marks; i += kSortThreads) reinterpret_cast<uint32_t *>(mark)[i] = 0;
@@ -347,28 +381,32 @@ __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const I *ids, i
 }
 
 // ---------------------------------------------------------------------------------------- gradient
-constexpr int kChunk = 32;      // sorted tokens of a block
+constexpr int kMaxChunk = 128;  // sorted tokens of a block, at most
 constexpr int kInFlight = 8;    // rows' loads of a thread in flight
 
 // The first blocks sum runs: block (chunk k, column tile) walks its tokens in order.  A run that lies in the chunk goes
 // to the table; part[2 k] takes the sum of one that came in from chunk k - 1 (and may go on), part[2 k + 1]
-// of one that starts here and goes on.  The other blocks write the rows that do not occur, kAccesses
-// accesses a thread: reads and writes of the two kinds overlap.
+// of one that starts here and goes on.  The other blocks write the rows that do not occur (from access `zeroed`
+// on), kAccesses accesses a thread.  Every `stride`-th block is one of the first kind: reads and writes
+// overlap.
 template <class T, class O, int VEC>
 __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout, RowMap dm, const uint32_t *key, const uint32_t *pos,
                                                                   uint32_t tokens, const uint8_t *mark, acc_t<T> *part,
                                                                   acc_t<T> scale, O *dtable, int64_t ld, uint32_t vocab,
-                                                                  RowSequence seq, uint32_t sum_blocks, FastDiv32 tiles)
+                                                                  RowSequence seq, uint32_t sum_blocks, FastDiv32 tiles,
+                                                                  FastDiv32 stride, int64_t zeroed, uint32_t chunk)
 {
     using A = acc_t<T>;
     using V = vec_t<T, VEC>;
     using VO = vec_t<O, VEC>;
     using Vals = Values<A, VEC>;
     cudaGridDependencySynchronize();
-    if (blockIdx.x >= sum_blocks) {
+    uint32_t block, off;
+    stride.divmod(blockIdx.x, block, off);
+    if (off != 0 || block >= sum_blocks) {
         int64_t row;
         uint32_t rest;
-        seq.start(int64_t(blockIdx.x - sum_blocks) * (kThreads * kAccesses), row, rest);
+        seq.start(zeroed + int64_t(blockIdx.x - min(block + (off != 0), sum_blocks)) * (kThreads * kAccesses), row, rest);
         Vals zero;
         zero.fill(0);
         const VO z = repack<O, VEC, A>(zero);
@@ -381,11 +419,11 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
         }
         return;
     }
-    __shared__ uint32_t keys[kChunk + 2];   // with the token before and the token behind the chunk
-    __shared__ int64_t rows[kChunk];
+    __shared__ uint32_t keys[kMaxChunk + 2];   // with the token before and the token behind the chunk
+    __shared__ int64_t rows[kMaxChunk];
     uint32_t k, tile;
-    tiles.divmod(blockIdx.x, k, tile);
-    const uint32_t begin = k * kChunk, count = min(tokens - begin, uint32_t(kChunk));
+    tiles.divmod(block, k, tile);
+    const uint32_t begin = k * chunk, count = min(tokens - begin, chunk);
     if (threadIdx.x < count + 2) {
         const int64_t i = int64_t(begin) + threadIdx.x - 1;
         keys[threadIdx.x] = i >= 0 && i < tokens ? key[i] : ~0u;
@@ -426,11 +464,12 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
 // Runs over several chunks: the block of the chunk in which one ends adds its parts in order.
 template <class A, class O, int VEC>
 __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t *key, uint32_t tokens, const A *part, A scale,
-                                                                  O *dtable, int64_t ld, uint32_t vocab, uint32_t per_row)
+                                                                  O *dtable, int64_t ld, uint32_t vocab, uint32_t per_row,
+                                                                  uint32_t chunk)
 {
     using Vals = Values<A, VEC>;
     cudaGridDependencySynchronize();
-    const uint32_t k = blockIdx.x + 1, begin = k * kChunk, end = min(tokens, begin + kChunk);
+    const uint32_t k = blockIdx.x + 1, begin = k * chunk, end = min(tokens, begin + chunk);
     const uint32_t id = key[begin];
     // a run that came in and ends here
     if (id >= vocab || key[begin - 1] != id || (end < tokens && key[end - 1] == id && key[end] == id)) return;
@@ -439,7 +478,7 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t
     uint32_t first = k;   // the first chunk that the run came into
     for (;;) {
         const int64_t at = int64_t(first) - 1 - (threadIdx.x & 31);   // chunk `at` passes the run on to at + 1
-        const unsigned on = __ballot_sync(0xffffffffu, at >= 1 && key[at * kChunk - 1] == id);
+        const unsigned on = __ballot_sync(0xffffffffu, at >= 1 && key[at * chunk - 1] == id);
         const int run = on == 0xffffffffu ? 32 : __ffs(~on) - 1;
         first -= run;
         if (run < 32) break;
@@ -492,21 +531,36 @@ static int64_t sort_words(int64_t n)   // of the sort's workspace
     return 4 * n + 4 * ceil_div(n, kTile) * kMaxDigits;
 }
 
+// Zeros that a launch of the sort writes on the side: what the memory takes in the 5 (counting) and 10 (placing)
+// us that the sort's own blocks need.
+constexpr int64_t kZerosCounting = int64_t(32) << 20, kZerosPlacing = int64_t(64) << 20;
+
+// Moves `zero` on to the next launch's share, of `bytes` at most; its number of blocks.
+static int64_t take_zeros(ZeroRows &z, int64_t bytes)
+{
+    z.first += z.blocks * (kThreads * kAccesses);
+    const int64_t left = std::max<int64_t>(0, z.rows * z.seq.per_row.d - z.first);
+    z.blocks = ceil_div(std::min(left, bytes / z.access), kThreads * kAccesses);
+    return z.blocks;
+}
+
 // Sorted keys and positions of the ids in `work` (two pairs of arrays of `n`, then the counters of the passes), and
 // marks of the ids that occur.
 template <class I> static void sort_ids(const void *ids, int64_t n, int64_t vocab, uint32_t *work, uint8_t *mark, uint32_t *&key,
-                                        uint32_t *&pos, cudaStream_t s)
+                                        uint32_t *&pos, ZeroRows &zero, cudaStream_t s)
 {
     int bits = 1;
     while ((int64_t(1) << bits) <= vocab) ++bits;
     const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes;
     const int64_t tiles = std::max<int64_t>(1, ceil_div(n, kTile)), counters = tiles << width, marks = ceil_div(vocab, 4);
-    const unsigned grid = static_cast<unsigned>(tiles), block = kSortThreads;
+    const unsigned block = kSortThreads;
+    const auto grid = [&](int64_t bytes) { return static_cast<unsigned>(tiles + take_zeros(zero, bytes)); };
     if (tiles == 1) {
         key = work;
         pos = work + n;
-        launch_after_previous(sort_tile_kernel<I>, grid, block, s, static_cast<const I *>(ids), n, vocab, passes, width, key, pos, mark,
-                              marks);
+        const unsigned blocks = grid(kZerosPlacing);
+        launch_after_previous(sort_tile_kernel<I>, blocks, block, s, static_cast<const I *>(ids), n, vocab, passes, width, key, pos, mark,
+                              marks, zero);
         note_kernel("sort_tile");
         return;
     }
@@ -520,21 +574,24 @@ template <class I> static void sort_ids(const void *ids, int64_t n, int64_t voca
         pos = bufs[p & 1][1];
         uint8_t *last = p + 1 == passes ? mark : nullptr;
         if (!joined || p == 0) {
-            launch_after_previous(sort_count_kernel<I>, grid, block, s, in, p == 0, n, vocab, shift, width, hist, joined ? passes - 1 : 0,
-                                  reinterpret_cast<uint32_t *>(mark), p == 0 ? marks : 0);
+            const unsigned blocks = grid(kZerosCounting);
+            launch_after_previous(sort_count_kernel<I>, blocks, block, s, in, p == 0, n, vocab, shift, width, hist, int(tiles),
+                                  joined ? passes - 1 : 0, reinterpret_cast<uint32_t *>(mark), p == 0 ? marks : 0, zero);
             note_kernel("sort_count");
         }
         if (joined) {
             uint32_t *next = p + 1 < passes ? hist + counters : nullptr;
-            launch_after_previous(sort_place_kernel<I, true>, grid, block, s, in, p == 0, n, vocab, shift, width, hist, next, key, pos,
-                                  last);
+            const unsigned blocks = grid(kZerosPlacing);
+            launch_after_previous(sort_place_kernel<I, true>, blocks, block, s, in, p == 0, n, vocab, shift, width, hist, next, key, pos,
+                                  last, int(tiles), zero);
             hist += counters;
         }
         else {
             launch_after_previous(sort_scan_kernel, 1u, unsigned(kMaxDigits), s, hist, tiles, 1 << width);
             note_kernel("sort_scan");
-            launch_after_previous(sort_place_kernel<I, false>, grid, block, s, in, p == 0, n, vocab, shift, width, hist,
-                                  static_cast<uint32_t *>(nullptr), key, pos, last);
+            const unsigned blocks = grid(kZerosPlacing);
+            launch_after_previous(sort_place_kernel<I, false>, blocks, block, s, in, p == 0, n, vocab, shift, width, hist,
+                                  static_cast<uint32_t *>(nullptr), key, pos, last, int(tiles), zero);
         }
         note_kernel("sort_place");
         in = {nullptr, key, pos};
@@ -548,18 +605,31 @@ struct EmbedGradArgs {
     double scale;
 };
 
-template <class T, class O, int VEC>
-static void launch_sums(const EmbedGradArgs &a, const uint32_t *key, const uint32_t *pos, const uint8_t *mark, acc_t<T> *part,
-                        cudaStream_t s)
+template <class T, class O, int VEC> static void run_sums(const EmbedGradArgs &a, void *work, size_t head, uint32_t chunk, cudaStream_t s)
 {
     using A = acc_t<T>;
-    const int64_t per_row = a.n / VEC, tiles = ceil_div(per_row, kThreads), chunks = ceil_div(a.tokens, kChunk);
+    uint32_t *w = static_cast<uint32_t *>(work), *key = nullptr, *pos = nullptr;
+    uint8_t *mark = reinterpret_cast<uint8_t *>(w + sort_words(a.tokens));
+    A *part = reinterpret_cast<A *>(static_cast<char *>(work) + head);
+    const int64_t per_row = a.n / VEC, tiles = ceil_div(per_row, kThreads), chunks = ceil_div(a.tokens, int64_t(chunk));
     O *dtable = static_cast<O *>(a.dtable->data);
-    launch_after_previous(embedding_sums_kernel<T, O, VEC>, static_cast<unsigned>(chunks * tiles) + sequence_blocks(a.vocab, per_row),
-                          unsigned(kThreads), s, static_cast<const T *>(a.dout->data), a.dm, key, pos, uint32_t(a.tokens), mark, part,
-                          A(a.scale), dtable, a.ld, uint32_t(a.vocab), RowSequence{FastDiv32(uint32_t(per_row))},
-                          uint32_t(chunks * tiles), FastDiv32(uint32_t(tiles)));
-    note_kernel("embedding_sums");
+    // (a float32 gradient of float16 data takes two of these accesses for each of the sums')
+    constexpr int access = VEC * sizeof(O) > 16 ? 16 : VEC * static_cast<int>(sizeof(O));
+    ZeroRows zero = {reinterpret_cast<char *>(dtable), a.ld * int64_t(sizeof(O)), access,
+                     {FastDiv32(uint32_t(a.n * sizeof(O) / access))}, a.vocab, 0, 0};
+    if (a.ids->typenum == DPB_INT32) sort_ids<int32_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, zero, s);
+    else sort_ids<int64_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, zero, s);
+    take_zeros(zero, 0);
+    const int64_t zeroed = std::min(a.vocab * per_row, zero.first * access / int64_t(VEC * sizeof(O)));
+    const int64_t sums = chunks * tiles, zeros = ceil_div(a.vocab * per_row - zeroed, kThreads * kAccesses);
+    if (sums + zeros > 0) {
+        const int64_t stride = sums > 0 ? std::max<int64_t>(1, (sums + zeros) / sums) : 1;
+        launch_after_previous(embedding_sums_kernel<T, O, VEC>, static_cast<unsigned>(sums + zeros), unsigned(kThreads), s,
+                              static_cast<const T *>(a.dout->data), a.dm, key, pos, uint32_t(a.tokens), mark, part, A(a.scale), dtable,
+                              a.ld, uint32_t(a.vocab), RowSequence{FastDiv32(uint32_t(per_row))}, uint32_t(sums),
+                              FastDiv32(uint32_t(tiles)), FastDiv32(uint32_t(stride)), zeroed, chunk);
+        note_kernel("embedding_sums");
+    }
     if (chunks < 2) return;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(chunks - 1), static_cast<unsigned>(tiles));
@@ -572,31 +642,29 @@ static void launch_sums(const EmbedGradArgs &a, const uint32_t *key, const uint3
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    cudaLaunchKernelEx(&cfg, embedding_join_kernel<A, O, VEC>, key, uint32_t(a.tokens), static_cast<const A *>(part), A(a.scale), dtable,
-                       a.ld, uint32_t(a.vocab), uint32_t(per_row));
+    cudaLaunchKernelEx(&cfg, embedding_join_kernel<A, O, VEC>, static_cast<const uint32_t *>(key), uint32_t(a.tokens),
+                       static_cast<const A *>(part), A(a.scale), dtable, a.ld, uint32_t(a.vocab), uint32_t(per_row), chunk);
     note_kernel("embedding_join");
 }
 
 template <class T, class O> static int run_backward(const EmbedGradArgs &a, cudaStream_t s)
 {
     using A = acc_t<T>;
-    const int64_t chunks = ceil_div(a.tokens, kChunk);
-    const size_t words = static_cast<size_t>(sort_words(a.tokens) + ceil_div(a.vocab, 4)) * 4;   // then a mark a row
-    const size_t head = (words + 255) / 256 * 256;
-    void *work = nullptr;
-    DPB_TRY(dpb_malloc(head + static_cast<size_t>(2 * chunks * a.n) * sizeof(A), s, &work));
-    uint32_t *w = static_cast<uint32_t *>(work), *key = nullptr, *pos = nullptr;
-    uint8_t *mark = reinterpret_cast<uint8_t *>(w + sort_words(a.tokens));
-    A *part = reinterpret_cast<A *>(static_cast<char *>(work) + head);
-    if (a.ids->typenum == DPB_INT32) sort_ids<int32_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, s);
-    else sort_ids<int64_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, s);
     constexpr int wide = vec_width<T>();
     int v = a.tokens > 0 ? row_vector(a.dout->data, a.dm, a.n, sizeof(T), wide) : wide;
-    // (a float32 gradient of float16 data is written in accesses of at most 32 bytes)
     while (v > 1 && (a.n % v || a.ld % v || !is_aligned(a.dtable->data, v * sizeof(O)))) v /= 2;
-    if (v == wide) launch_sums<T, O, wide>(a, key, pos, mark, part, s);
-    else if (is_half_v<T> && v >= 2) launch_sums<T, O, is_half_v<T> ? 2 : 1>(a, key, pos, mark, part, s);
-    else launch_sums<T, O, 1>(a, key, pos, mark, part, s);
+    // long chunks leave fewer parts of frequent ids to add up, short ones give few tokens enough blocks
+    const int64_t tiles = ceil_div(ceil_div(a.n, v), kThreads);
+    uint32_t chunk = 32;
+    while (chunk < kMaxChunk && a.tokens / (2 * chunk) * tiles >= 4 * device_props().sm_count) chunk *= 2;
+    // sorted keys and positions, counters, a mark a row; parts of runs
+    const size_t words = static_cast<size_t>(sort_words(a.tokens) + ceil_div(a.vocab, 4)) * 4;
+    const size_t head = (words + 255) / 256 * 256;
+    void *work = nullptr;
+    DPB_TRY(dpb_malloc(head + static_cast<size_t>(2 * ceil_div(a.tokens, int64_t(chunk)) * a.n) * sizeof(A), s, &work));
+    if (v == wide) run_sums<T, O, wide>(a, work, head, chunk, s);
+    else if (is_half_v<T> && v >= 2) run_sums<T, O, is_half_v<T> ? 2 : 1>(a, work, head, chunk, s);
+    else run_sums<T, O, 1>(a, work, head, chunk, s);
     const int st = check_launch("embedding_backward");
     dpb_free(work, s);
     return st;
