@@ -108,10 +108,11 @@ inline bool wide_ok(const void *p, int vec, int item)
     return !p || is_aligned(p, static_cast<size_t>(bytes > 16 ? 16 : bytes));
 }
 
-// launch_after_previous with dynamic shared memory.  A block of more than 48 KiB in all has to ask
-// for it.
+// launch_after_previous with dynamic shared memory (a block of more than 48 KiB in all has to ask for it) and
+// clusters of `cluster` blocks.
 template <class... KArgs, class... Args>
-inline void launch_shared(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t shared, cudaStream_t stream, Args... args)
+inline void launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned cluster, unsigned block, size_t shared,
+                           cudaStream_t stream, Args... args)
 {
     if (shared > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
     cudaLaunchConfig_t cfg = {};
@@ -119,14 +120,24 @@ inline void launch_shared(void (*kernel)(KArgs...), unsigned grid, unsigned bloc
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = shared;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
     if (tuning_pdl()) {
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
     cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);   // an error stays in cudaGetLastError for check_launch
+}
+template <class... KArgs, class... Args>
+inline void launch_shared(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t shared, cudaStream_t stream, Args... args)
+{
+    launch_cluster(kernel, grid, 1u, block, shared, stream, args...);
 }
 
 // -------------------------------------------------------------------------------- argument checks
