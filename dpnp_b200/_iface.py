@@ -433,18 +433,31 @@ def any(a, /, axis=None, out=None, keepdims=False, *, where=True):
 
 
 # ----------------------------------------------------------- row operators
+_PASSED = (type(None), int, float)
+
+
+def _row_arg(a):
+    """A public array's tensor; None and numbers as they are."""
+    t = type(a)
+    if t is dpnp_array:
+        return a._array_obj
+    return a if t in _PASSED or isinstance(a, (int, float, np.generic)) else get_usm_ndarray(a)
+
+
 def _row_call(fn, arrays, out, **kwargs):
     """A row operator of the tensor layer on public arrays: results are public arrays, an `out` array itself
-    where one was given (numbers and None among `arrays` pass through)."""
-    usm = [a if a is None or isinstance(a, (int, float, np.generic)) else get_usm_ndarray(a) for a in arrays]
-    several = isinstance(out, (tuple, list))
-    usm_out = type(out)(None if o is None else get_usm_ndarray(o) for o in out) if several \
-        else None if out is None else get_usm_ndarray(out)
-    res = fn(*usm, out=usm_out, **kwargs)
-    if not isinstance(res, tuple):
-        return _wrap(res) if out is None or isinstance(out, usm_ndarray) else out
-    given = out if several else (None,) * len(res)
-    return tuple(o if isinstance(o, dpnp_array) else _wrap(r) for o, r in zip(given, res))
+    where one was given."""
+    usm = [_row_arg(a) for a in arrays]
+    if out is None:
+        res = fn(*usm, **kwargs)
+        return tuple([_wrap(r) for r in res]) if type(res) is tuple else _wrap(res)
+    if isinstance(out, (tuple, list)):
+        res = fn(*usm, out=tuple([None if o is None else get_usm_ndarray(o) for o in out]), **kwargs)
+        if type(res) is not tuple:
+            return _wrap(res)
+        return tuple([o if type(o) is dpnp_array else _wrap(r) for o, r in zip(out, res)])
+    res = fn(*usm, out=get_usm_ndarray(out), **kwargs)
+    return _wrap(res) if isinstance(out, usm_ndarray) else out
 
 
 def layer_norm(x, weight=None, bias=None, /, *, axis=-1, eps=1e-5, return_stats=False, out=None):

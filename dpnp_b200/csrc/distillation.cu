@@ -38,14 +38,51 @@ template <bool FTZ> DPB_D float exp2_(float a)
 template <bool FTZ> DPB_D double exp2_(double a) { return exp2(a); }
 constexpr double kLog2E = 1.4426950408889634074;
 
-// The largest value and the sum of exp((v - largest) / T) of some values, T given as k = log2(e) / T.
-template <class A> struct alignas(2 * sizeof(A)) SoftSum {
-    A top, sum;
-    // what v is reduced by: a finite number even where every value is -inf
+// Exponentials of a row's values below its largest one, T given as k = log2(e) / T.
+//
+// float and double: 2^((v - top) k), the difference taken first, so that values of the type's lowest number do not
+// overflow.  float16: 2^(v k - c) with c = top k rounded, which is one fused operation a value; what c is off by
+// (rest) is exact and corrects the sum once.  `finite`: what a row whose values are all -inf is reduced by.
+template <class T> struct Exponent {
+    using A = acc_t<T>;
+    static constexpr bool fused = is_half_v<T>;
+    A k, base;
     static DPB_D A finite(A t) { return t == -INFINITY ? A(0) : t; }
+    DPB_D Exponent(A top, A k_) : k(k_), base(fused ? -(finite(top) * k_) : -finite(top)) {}
+    template <bool FTZ> DPB_D A exp(A v) const
+    {
+        return exp2_<FTZ>(fused ? fma_(v, k, base) : (v + base) * k);
+    }
+    template <bool FTZ, int N> DPB_D void exp(Values<A, N> &v) const
+    {
+        Values<A, N> e;
+        if constexpr (fused) {
+            e.fill(base);
+            e.fma_add(v, k);
+        }
+        else {
+            e = v;
+            e.add(base);
+            e.mul(k);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v.set(i, exp2_<FTZ>(e.get(i)));
+    }
+    // log2 of the factor between the sum of these exponentials and that of exp((v - top) / T)
+    DPB_D A rest(A top) const { return fused ? fma_(finite(top), k, base) : A(0); }
+};
+
+// The largest of some values and the sum of their exponentials.
+template <class T> struct alignas(2 * sizeof(acc_t<T>)) SoftSum {
+    using A = acc_t<T>;
+    A top, sum;
     DPB_D void raise(A to, A k)   // to >= top
     {
-        sum *= exp2_<true>((top - finite(to)) * k);
+        if constexpr (Exponent<T>::fused) {
+            const A factor = exp2_<true>(Exponent<T>(to, k).base - Exponent<T>(top, k).base);
+            sum = top == -INFINITY ? A(0) : sum * factor;
+        }
+        else sum *= exp2_<true>((top - Exponent<T>::finite(to)) * k);
         top = to;
     }
     DPB_D SoftSum over_warp(A k) const
@@ -55,7 +92,29 @@ template <class A> struct alignas(2 * sizeof(A)) SoftSum {
         s.sum = warp_fold(SumF(), s.sum);
         return s;
     }
+    DPB_D A log_sum(A k) const   // log sum exp((v - top) / T)
+    {
+        return log_(sum) - Exponent<T>(top, k).rest(top) * A(0.69314718055994530942);
+    }
 };
+
+// Largest of the values of an access, NaN if there is one.
+template <class T, int N> DPB_D acc_t<T> largest(const vec_t<T, N> &raw)
+{
+    if constexpr (is_half_v<T>) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(raw.v);
+        __half2 m = h[0];
+#pragma unroll
+        for (int i = 1; i < N / 2; ++i) m = __hmax2_nan(m, h[i]);
+        return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+    }
+    else {
+        acc_t<T> m = raw.v[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = max_nan(m, raw.v[i]);
+        return m;
+    }
+}
 
 // A row's teacher as a block keeps it: probability, its logarithm and column (-1: does not count) of each entry.
 template <class A> struct Teacher {
@@ -64,7 +123,7 @@ template <class A> struct Teacher {
     static DPB_HD size_t bytes(int k) { return size_t(k) * (2 * sizeof(A) + sizeof(int)) + 16; }
     DPB_D Teacher(void *shared, int k) : p(static_cast<A *>(shared)), logp(p + k), at(reinterpret_cast<int *>(logp + k)) {}
     // One warp reads the entries; false when none counts.
-    template <class I> DPB_D bool read(const A *top, const I *index, int k, int64_t vocab) const
+    template <class I> DPB_D bool read(const A *top, const I *index, int k, int vocab) const
     {
         bool any = false;
         for (int i = threadIdx.x & 31; i < k; i += 32) {
@@ -111,177 +170,227 @@ template <class A> struct Teacher {
     }
 };
 
-// A row of V logits as whole accesses of 16 bytes behind `head` single elements, `tail` elements behind them; a
-// rank (of `ranks` blocks) has `mine` accesses from access `begin` on.
+// How rows are shared out: 2^bits blocks (ranks) a row, `each` accesses a rank at most.
+struct Shares {
+    int bits, each;
+    DPB_D uint32_t row() const { return blockIdx.x >> bits; }
+    DPB_D int rank() const { return blockIdx.x & ((1 << bits) - 1); }
+};
+
+// A row of V logits as whole accesses of 16 bytes behind `head` single elements, `tail` elements behind them; a rank has
+// `mine` accesses, the first of which starts at column `first`.
 template <class T> struct RowSplit {
     static constexpr int VEC = vec_width<T>();
-    int head, tail;
-    int64_t begin, mine;
-    DPB_D RowSplit(const T *row, int64_t vocab, int rank, int ranks)
+    int head, tail, first, mine;
+    DPB_D RowSplit(const T *row, int vocab, const Shares &sh)
     {
-        const int off = misalignment(row);
-        head = static_cast<int>(min(vocab, int64_t(off ? VEC - off : 0)));
-        const int64_t all = (vocab - head) / VEC, each = (all + ranks - 1) / ranks;
-        tail = static_cast<int>(vocab - head - all * VEC);
-        begin = min(all, each * rank);
-        mine = min(all, begin + each) - begin;
+        const int off = misalignment(row), rank = sh.rank();
+        head = min(vocab, off ? VEC - off : 0);
+        const int all = (vocab - head) / VEC, begin = min(all, sh.each * rank);
+        tail = vocab - head - all * VEC;
+        mine = min(all, begin + sh.each) - begin;
+        first = head + begin * VEC;
         if (rank > 0) head = 0;
-        if (rank < ranks - 1) tail = 0;
+        if (rank < (1 << sh.bits) - 1) tail = 0;
     }
     // The thread's single element (head or tail), as a column; -1 without one.
-    DPB_D int64_t single(int64_t vocab) const
+    DPB_D int single(int vocab) const
     {
         const int t = threadIdx.x;
         return t < head ? t : t < head + tail ? vocab - tail + (t - head) : -1;
     }
 };
 
-// The gradient of the columns from the row's statistics: q = 2^((z - top) k - log2 of the sum), in which a row
-// whose logits are all -inf counts as one of sum 1 (q is 0 then).
+// The gradient of a row's columns, dloss T (q - weight): q is an exponential times `scale` (0 in a row whose logits
+// are all -inf).
 template <class T> struct RowGradient {
     using A = acc_t<T>;
     static constexpr bool ftz = is_half_v<T>;   // (float16 has no numbers as small as those that are flushed)
-    A top, k, shift, g;
-    DPB_D RowGradient(A top_, A log_sum, A k_, A g_)
-        : top(SoftSum<A>::finite(top_)), k(k_), shift(log_sum == -INFINITY ? A(0) : -log_sum * A(kLog2E)), g(g_)
+    Exponent<T> ex;
+    A scale, g;
+    DPB_D RowGradient(const SoftSum<T> &s, A k, A g_) : ex(s.top, k), scale(s.sum == 0 ? A(0) : g_ / s.sum), g(g_) {}
+    DPB_D RowGradient(A top, A log_sum, A k, A g_)   // from kept statistics
+        : ex(top, k), scale(log_sum == -INFINITY ? A(0) : g_ * exp_(-log_sum) * exp2_<false>(-ex.rest(top))), g(g_)
     {
     }
-    DPB_D A q(A v) const { return exp2_<ftz>(fma_(v - top, k, shift)); }
+    DPB_D A at(A v, A weight) const { return ex.template exp<ftz>(v) * scale - g * weight; }
     template <int N> DPB_D void apply(Values<A, N> &v) const
     {
-        Values<A, N> e;
-        e.fill(shift);
-        v.add(-top);
-        e.fma_add(v, k);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v.set(i, exp2_<ftz>(e.get(i)));
-        v.mul(g);
+        ex.template exp<ftz>(v);
+        v.mul(scale);
     }
 };
 
-// ------------------------------------------------------------------------------ rows in shared memory
-// A cluster of 1 to 8 blocks takes a row and keeps it in its blocks' shared memory, so that the logits cross the
-// memory once for loss and gradient: copies of all accesses are queued at once in four groups, each group is
-// summed as it arrives (largest value and sum, both per thread), the blocks exchange their sums through
-// distributed shared memory, and (GRAD) every block writes the gradient of its part.  The threads read only what
-// they copied themselves, so that the copies need no barrier.
+// ------------------------------------------------------------------------------------------- a row's parts
+constexpr int kThreads = 256;   // of a block, at most
+constexpr int kInFlight = 4;    // accesses of a thread
+constexpr int kMaxRanks = 8;    // blocks of a cluster
+
+// What a block of either kernel below knows of its part of a row, and its work on it.
+template <class T, class I> struct RowPart {
+    using A = acc_t<T>;
+    static constexpr int VEC = vec_width<T>();
+    using V = vec_t<T, VEC>;
+    const T *row;
+    RowSplit<T> split;
+    Teacher<A> teacher;
+    A *at_teacher;   // the student's logits at the teacher's columns
+    int single, k, vocab;
+
+    static DPB_HD size_t shared_bytes(int k) { return (Teacher<A>::bytes(k) + 15) / 16 * 16 + size_t(k) * sizeof(A); }
+    DPB_D RowPart(const T *row_, int vocab_, int k_, const Shares &share, char *shared)
+        : row(row_), split(row_, vocab_, share), teacher(shared, k_),
+          at_teacher(reinterpret_cast<A *>(shared + (Teacher<A>::bytes(k_) + 15) / 16 * 16)), single(split.single(vocab_)), k(k_), vocab(vocab_)
+    {
+    }
+    DPB_D bool owns(int c) const
+    {
+        return (c >= split.first && c < split.first + split.mine * VEC) || (c >= 0 && c < split.head) || c >= vocab - split.tail;
+    }
+    // The first warp reads the teacher's entries.  Whether one counts, for the whole block.
+    DPB_D bool read_teacher(const A *top, const I *index, int &used) const
+    {
+        if (threadIdx.x < 32) {
+            const bool any = teacher.read(top, index, k, vocab);
+            if (threadIdx.x == 0) used = any;
+        }
+        __syncthreads();
+        return used;
+    }
+    // The first warp reads the logits at the teacher's columns (`all`, or this part's), before any block writes over them.
+    DPB_D void read_at_teacher(bool all) const
+    {
+        if (threadIdx.x >= 32) return;
+        for (int i = threadIdx.x; i < k; i += 32) {
+            const int c = teacher.at[i];
+            if (c >= 0 && (all || owns(c))) at_teacher[i] = to_acc<A>(row[c]);
+        }
+    }
+    DPB_D const V *from() const { return reinterpret_cast<const V *>(row + split.first); }
+    // Stores that are not read again here: they leave the cache first.
+    DPB_D void put(T *out, int i, const V &v, bool aligned) const
+    {
+        T *o = out + split.first + i * VEC;
+        if (aligned) __stcs(reinterpret_cast<int4 *>(o), reinterpret_cast<const int4 &>(v));
+        else
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) o[j] = v.v[j];
+    }
+    DPB_D bool aligned(const T *out) const { return split.mine > 0 && misalignment(out + split.first) == 0; }
+    DPB_D void zeros(T *out) const
+    {
+        const bool whole = aligned(out);
+        V z;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z.v[j] = from_acc<T>(A(0));
+        for (int i = threadIdx.x; i < split.mine; i += blockDim.x) put(out, i, z, whole);
+        if (single >= 0) out[single] = z.v[0];
+    }
+    DPB_D void dense_gradient(T *out, const RowGradient<T> &grad) const
+    {
+        const bool whole = aligned(out);
+        const int threads = blockDim.x;
+        const V *p = from();
+        for (int i0 = threadIdx.x; i0 < split.mine; i0 += kInFlight * threads) {
+            V raw[kInFlight];
+#pragma unroll
+            for (int f = 0; f < kInFlight; ++f)
+                if (i0 + f * threads < split.mine) raw[f] = p[i0 + f * threads];
+#pragma unroll
+            for (int f = 0; f < kInFlight; ++f) {
+                if (i0 + f * threads >= split.mine) break;
+                Values<A, VEC> v;
+                unpack<A, VEC, T>(raw[f], v);
+                grad.apply(v);
+                put(out, i0 + f * threads, repack<T, VEC, A>(v), whole);
+            }
+        }
+        if (single >= 0) out[single] = from_acc<T>(grad.at(to_acc<A>(row[single]), A(0)));
+    }
+    // The teacher's columns of this part once more, with its weight taken off (after a barrier).
+    DPB_D void teacher_gradient(T *out, const RowGradient<T> &grad) const
+    {
+        for (int i = threadIdx.x; i < k; i += blockDim.x) {
+            const int c = teacher.at[i];
+            if (c < 0 || !owns(c)) continue;
+            A weight;
+            if (teacher.first_of_column(i, k, weight)) out[c] = from_acc<T>(grad.at(at_teacher[i], weight));
+        }
+    }
+};
+
+// --------------------------------------------------------------------------------- loss, and loss and gradient
+// A cluster of 1 to 8 blocks takes a row: every block streams its part (largest value and sum of exponentials, both per
+// thread), the blocks exchange their sums through distributed shared memory, and (GRAD) read their parts again,
+// from the second-level cache, for the gradient: the logits cross the memory once.  The clusters that run at a
+// time hold 30 to 60 MB, which the cache keeps.  (The parts kept in shared memory instead, by copies that run ahead:
+// 487 us at 4096 x 128000 float16, because few threads fit beside them.)
 //
 // Two exponentials an element: at float16 and the copy rate that is 3.3e12 a second, three quarters of what the
 // special function units give; the rest of the arithmetic is done in pairs to stay out of their way.
-constexpr int kGroups = 4;      // groups of copies
-constexpr int kMaxRanks = 8;
-
 template <class T, class I, bool GRAD>
-__global__ void __launch_bounds__(512, 2)
-    distillation_row_kernel(const T *z, RowMap zm, const acc_t<T> *top, const I *index, int k, int64_t vocab, acc_t<T> temp,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
+    distillation_row_kernel(const T *z, RowMap zm, const acc_t<T> *top, const I *index, int k, int vocab, acc_t<T> temp,
                             acc_t<T> inv_temp, acc_t<T> exp_scale, acc_t<T> *loss, acc_t<T> *stats, const acc_t<T> *dloss,
-                            int64_t dstep, T *dz, RowMap dm, int ranks)
+                            int64_t dstep, T *dz, RowMap dm, Shares share)
 {
     using A = acc_t<T>;
-    constexpr int VEC = vec_width<T>();
-    using V = vec_t<T, VEC>;
+    using Part = RowPart<T, I>;
+    using V = typename Part::V;
+    constexpr int VEC = Part::VEC;
     extern __shared__ __align__(16) char shared_bytes[];
-    __shared__ SoftSum<A> warp_sums[16], rank_sums[kMaxRanks];
-    __shared__ A buf[32], singles[2 * VEC];
+    __shared__ SoftSum<T> warp_sums[kThreads / 32], rank_sums[kMaxRanks];
+    __shared__ A buf[kThreads / 32];
     __shared__ int used;
     cudaGridDependencySynchronize();
-    const uint32_t r = blockIdx.x / ranks;
-    const int rank = blockIdx.x % ranks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x;
-    const T *row = z + zm(r);
-    const RowSplit<T> part(row, vocab, rank, ranks);
-    const Teacher<A> teacher(shared_bytes, k);
-    V *slot = reinterpret_cast<V *>(shared_bytes + (Teacher<A>::bytes(k) + 15) / 16 * 16);
-    if (warp == 0) {
-        const bool any = teacher.read(top + int64_t(r) * k, index + int64_t(r) * k, k, vocab);
-        if (lane == 0) used = any;
-    }
-    __syncthreads();
+    const uint32_t r = share.row();
+    const int rank = share.rank(), ranks = 1 << share.bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x;
+    const Part part(z + zm(r), vocab, k, share, shared_bytes);
     T *out = GRAD ? dz + dm(r) : nullptr;
-    const int64_t first = part.begin * VEC + (rank == 0 ? part.head : misalignment(row) ? VEC - misalignment(row) : 0);
-    const int64_t single = part.single(vocab);
-    if (!used) {   // in every block of the cluster
+    if (!part.read_teacher(top + int64_t(r) * k, index + int64_t(r) * k, used)) {   // every block of the cluster
         if (rank == 0 && threadIdx.x == 0) {
             if (loss) loss[r] = 0;
             if (stats) stats[2 * int64_t(r)] = stats[2 * int64_t(r) + 1] = 0;
         }
-        if constexpr (GRAD) {
-            const bool aligned = part.mine > 0 && misalignment(out + first) == 0;
-            V zero;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) zero.v[j] = from_acc<T>(A(0));
-            for (int64_t i = threadIdx.x; i < part.mine; i += threads) {
-                T *o = out + first + i * VEC;
-                if (aligned) *reinterpret_cast<V *>(o) = zero;
-                else
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) o[j] = zero.v[j];
-            }
-            if (single >= 0) out[single] = zero.v[0];
-        }
+        if constexpr (GRAD) part.zeros(out);
         return;
     }
-    const int mine = static_cast<int>(part.mine), quarter = (mine + kGroups * threads - 1) / (kGroups * threads) * threads;
-    const V *from = reinterpret_cast<const V *>(row + first);
-    for (int g = 0; g < kGroups; ++g) {
-        const int end = min(mine, (g + 1) * quarter);
-        for (int i = g * quarter + threadIdx.x; i < end; i += threads) copy_async(slot + i, from + i);
-        copy_async_commit();
-    }
-    const A alone = single >= 0 ? to_acc<A>(row[single]) : A(-INFINITY);
-    if (single >= 0) singles[threadIdx.x] = alone;
-    A *at_teacher = reinterpret_cast<A *>(slot + mine);   // the student's logits at the teacher's columns
-    if (warp == 0) {
-        if (rank == 0)   // (read before any block writes over them)
-            for (int i = lane; i < k; i += 32)
-                if (teacher.at[i] >= 0) at_teacher[i] = to_acc<A>(row[teacher.at[i]]);
-        teacher.normalize(k, inv_temp);
-    }
-    SoftSum<A> s = {alone, single >= 0 && !(alone == -INFINITY) ? A(alone - alone + 1) : A(0)};
-    const auto take = [&](int begin, int end) {
-        constexpr int batch = 2;
-        for (int i = begin + threadIdx.x; i < end; i += batch * threads) {
-            Values<A, VEC> v[batch];
-            unpack<A, VEC, T>(slot[i], v[0]);
-            const bool more = i + threads < end;
-            if (more) unpack<A, VEC, T>(slot[i + threads], v[1]);
-            else v[1] = v[0];
-            A best = v[0].get(0);
+    const A alone = part.single >= 0 ? to_acc<A>(part.row[part.single]) : A(-INFINITY);
+    SoftSum<T> s = {alone, part.single >= 0 ? Exponent<T>(alone, exp_scale).template exp<true>(alone) : A(0)};
+    const V *from = part.from();
+    V low;
 #pragma unroll
-            for (int b = 0; b < batch; ++b)
+    for (int j = 0; j < VEC; ++j) low.v[j] = from_acc<T>(A(-INFINITY));
+    for (int i0 = threadIdx.x; i0 < part.split.mine; i0 += kInFlight * threads) {
+        V raw[kInFlight];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) best = max_nan(best, v[b].get(j));
-            s.raise(max_nan(s.top, best), exp_scale);
-            const A down = -SoftSum<A>::finite(s.top);
+        for (int f = 0; f < kInFlight; ++f) raw[f] = i0 + f * threads < part.split.mine ? from[i0 + f * threads] : low;
+        A best = largest<T, VEC>(raw[0]);
 #pragma unroll
-            for (int b = 0; b < batch; ++b) {
-                if (b > 0 && !more) break;
-                v[b].add(down);
-                v[b].mul(exp_scale);
-                auto sum = Values<A, VEC>::all(0);
-                Values<A, VEC> e;
+        for (int f = 1; f < kInFlight; ++f) best = max_nan(best, largest<T, VEC>(raw[f]));
+        s.raise(max_nan(s.top, best), exp_scale);
+        const Exponent<T> ex(s.top, exp_scale);
+        auto sum = Values<A, VEC>::all(0);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) e.set(j, exp2_<true>(v[b].get(j)));
-                e.sum_into(sum);
-                s.sum += Values<A, VEC>::join(sum);
-            }
+        for (int f = 0; f < kInFlight; ++f) {
+            Values<A, VEC> v;
+            unpack<A, VEC, T>(raw[f], v);
+            ex.template exp<true>(v);
+            v.sum_into(sum);
         }
-    };
-    copy_async_wait<3>();
-    take(0, min(mine, quarter));
-    copy_async_wait<2>();
-    take(quarter, min(mine, 2 * quarter));
-    copy_async_wait<1>();
-    take(2 * quarter, min(mine, 3 * quarter));
-    copy_async_wait<0>();
-    take(3 * quarter, mine);
+        s.sum += Values<A, VEC>::join(sum);
+    }
+    part.read_at_teacher(rank == 0);
+    if (warp == 0) part.teacher.normalize(k, inv_temp);
     // lanes, warps and ranks, each in a fixed order
     s = s.over_warp(exp_scale);
     if (lane == 0) warp_sums[warp] = s;
     __syncthreads();
-    s = lane < threads / 32 ? warp_sums[lane] : SoftSum<A>{-INFINITY, 0};
+    s = lane < threads / 32 ? warp_sums[lane] : SoftSum<T>{-INFINITY, 0};
     s = s.over_warp(exp_scale);
     if (ranks > 1) {
-        // every rank writes its sum to every rank; the barrier of the cluster makes them visible
+        // every rank writes its sum to every rank; the barrier of the cluster makes them visible (and follows the reads
+        // of read_at_teacher)
         if (threadIdx.x < ranks) {
             const uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(&rank_sums[rank]));
             uint32_t remote;
@@ -293,16 +402,17 @@ __global__ void __launch_bounds__(512, 2)
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        s = lane < ranks ? rank_sums[lane] : SoftSum<A>{-INFINITY, 0};
+        s = lane < ranks ? rank_sums[lane] : SoftSum<T>{-INFINITY, 0};
         s = s.over_warp(exp_scale);
     }
-    const A log_sum = log_(s.sum);
     if (rank == 0) {
+        const A log_sum = s.log_sum(exp_scale);
         A total = 0;
-        for (int i = threadIdx.x; i < k; i += threads) {
-            if (teacher.at[i] < 0 || teacher.p[i] == 0) continue;
-            const A v = at_teacher[i];
-            total += teacher.p[i] * (teacher.logp[i] - (v == -INFINITY ? A(-INFINITY) : (v - s.top) * inv_temp - log_sum));
+        for (int i = threadIdx.x; i < k; i += blockDim.x) {
+            if (part.teacher.at[i] < 0 || part.teacher.p[i] == 0) continue;
+            const A v = part.at_teacher[i];
+            total += part.teacher.p[i] *
+                     (part.teacher.logp[i] - (v == -INFINITY ? A(-INFINITY) : (v - s.top) * inv_temp - log_sum));
         }
         total = block_fold(SumF(), total, buf);
         if (threadIdx.x == 0) {
@@ -314,171 +424,36 @@ __global__ void __launch_bounds__(512, 2)
         }
     }
     if constexpr (GRAD) {
-        const RowGradient<T> grad(s.top, log_sum, exp_scale, dloss[r * dstep] * temp);
-        const bool aligned = mine > 0 && misalignment(out + first) == 0;
-        for (int i = threadIdx.x; i < mine; i += threads) {
-            Values<A, VEC> v;
-            unpack<A, VEC, T>(slot[i], v);
-            grad.apply(v);
-            const V w = repack<T, VEC, A>(v);
-            T *o = out + first + int64_t(i) * VEC;
-            if (aligned) *reinterpret_cast<V *>(o) = w;
-            else
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) o[j] = w.v[j];
-        }
-        if (single >= 0) out[single] = from_acc<T>(grad.g * grad.q(alone));
+        const RowGradient<T> grad(s, exp_scale, dloss[r * dstep] * temp);
+        part.dense_gradient(out, grad);
         __syncthreads();
-        // the teacher's columns of this block's part once more, with its weight taken off
-        const T *values = reinterpret_cast<const T *>(slot);
-        for (int i = threadIdx.x; i < k; i += threads) {
-            const int64_t c = teacher.at[i];
-            if (c < 0) continue;
-            const bool inside = c >= first && c < first + int64_t(mine) * VEC;
-            if (!inside && !(c < part.head || c >= vocab - part.tail)) continue;
-            A weight;
-            if (!teacher.first_of_column(i, k, weight)) continue;
-            if (inside) out[c] = from_acc<T>(grad.g * (grad.q(to_acc<A>(values[c - first])) - weight));
-            else out[c] = from_acc<T>(grad.g * (grad.q(singles[c < part.head ? c : part.head + (c - (vocab - part.tail))]) - weight));
-        }
+        part.teacher_gradient(out, grad);
     }
 }
 
 // ------------------------------------------------------------------------------------------ gradient alone
-// From kept statistics: `ranks` blocks a row, each a part of it, four accesses of a thread in flight.
-constexpr int kThreads = 256;
-
+// From kept statistics: the same parts, without exchange.
 template <class T, class I>
 __global__ void __launch_bounds__(kThreads)
     distillation_grad_kernel(const acc_t<T> *dloss, int64_t dstep, const T *z, RowMap zm, const acc_t<T> *top, const I *index, int k,
-                             int64_t vocab, acc_t<T> temp, acc_t<T> inv_temp, acc_t<T> exp_scale, const acc_t<T> *stats, T *dz,
-                             RowMap dm, int ranks)
+                             int vocab, acc_t<T> temp, acc_t<T> inv_temp, acc_t<T> exp_scale, const acc_t<T> *stats, T *dz,
+                             RowMap dm, Shares share)
 {
     using A = acc_t<T>;
-    constexpr int VEC = vec_width<T>(), flight = 4;
-    using V = vec_t<T, VEC>;
     extern __shared__ __align__(16) char shared_bytes[];
     __shared__ int used;
     cudaGridDependencySynchronize();
-    const uint32_t r = blockIdx.x / ranks;
-    const int rank = blockIdx.x % ranks;
-    const T *row = z + zm(r);
+    const uint32_t r = share.row();
+    const RowPart<T, I> part(z + zm(r), vocab, k, share, shared_bytes);
     T *out = dz + dm(r);
-    const RowSplit<T> part(row, vocab, rank, ranks);
-    const int64_t first = part.begin * VEC + (rank == 0 ? part.head : misalignment(row) ? VEC - misalignment(row) : 0);
-    const int64_t last = first + part.mine * VEC, single = part.single(vocab);
-    const Teacher<A> teacher(shared_bytes, k);
-    A *at_teacher = reinterpret_cast<A *>(shared_bytes + (Teacher<A>::bytes(k) + 15) / 16 * 16);
-    if (threadIdx.x < 32) {
-        const bool any = teacher.read(top + int64_t(r) * k, index + int64_t(r) * k, k, vocab);
-        if (threadIdx.x == 0) used = any;
-        for (int i = threadIdx.x; i < k; i += 32) {   // before the block writes over them
-            const int64_t c = teacher.at[i];
-            const bool mine = c >= 0 && ((c >= first && c < last) || c < part.head || c >= vocab - part.tail);
-            if (mine) at_teacher[i] = to_acc<A>(row[c]);
-            else teacher.at[i] = c < 0 ? -1 : -2 - static_cast<int>(c);   // counts, in another block's part
-        }
-    }
+    if (!part.read_teacher(top + int64_t(r) * k, index + int64_t(r) * k, used)) return part.zeros(out);
+    part.read_at_teacher(false);
     __syncthreads();
-    const bool counts = used;
-    const RowGradient<T> grad(counts ? stats[2 * int64_t(r)] : A(0), counts ? stats[2 * int64_t(r) + 1] : A(0), exp_scale,
-                              dloss[r * dstep] * temp);
-    const bool aligned = part.mine > 0 && misalignment(out + first) == 0;
-    const auto put = [&](int64_t i, const V &w) {
-        T *o = out + first + i * VEC;
-        if (aligned) *reinterpret_cast<V *>(o) = w;
-        else
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = w.v[j];
-    };
-    const V *from = reinterpret_cast<const V *>(row + first);
-    V zero;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) zero.v[j] = from_acc<T>(A(0));
-    for (int64_t i0 = threadIdx.x; i0 < part.mine; i0 += flight * kThreads) {
-        V raw[flight];
-#pragma unroll
-        for (int f = 0; f < flight; ++f)
-            if (counts && i0 + f * kThreads < part.mine) raw[f] = from[i0 + f * kThreads];
-#pragma unroll
-        for (int f = 0; f < flight; ++f) {
-            if (i0 + f * kThreads >= part.mine) break;
-            if (!counts) {
-                put(i0 + f * kThreads, zero);
-                continue;
-            }
-            Values<A, VEC> v;
-            unpack<A, VEC, T>(raw[f], v);
-            grad.apply(v);
-            put(i0 + f * kThreads, repack<T, VEC, A>(v));
-        }
-    }
-    if (single >= 0) out[single] = counts ? from_acc<T>(grad.g * grad.q(to_acc<A>(row[single]))) : zero.v[0];
-    if (!counts) return;
-    if (threadIdx.x < 32) {
-        // all entries that count take part in the probabilities
-        for (int i = threadIdx.x; i < k; i += 32)
-            if (teacher.at[i] < -1) teacher.at[i] = -2 - teacher.at[i];
-        __syncwarp();
-        teacher.normalize(k, inv_temp);
-    }
+    const RowGradient<T> grad(stats[2 * int64_t(r)], stats[2 * int64_t(r) + 1], exp_scale, dloss[r * dstep] * temp);
+    part.dense_gradient(out, grad);
+    if (threadIdx.x < 32) part.teacher.normalize(k, inv_temp);
     __syncthreads();
-    for (int i = threadIdx.x; i < k; i += kThreads) {
-        const int64_t c = teacher.at[i];
-        if (c < 0 || !((c >= first && c < last) || c < part.head || c >= vocab - part.tail)) continue;
-        A weight;
-        if (teacher.first_of_column(i, k, weight)) out[c] = from_acc<T>(grad.g * (grad.q(at_teacher[i]) - weight));
-    }
-}
-
-// Rows beyond the shared memory of a cluster: one block a row, read twice.
-template <class T, class I>
-__global__ void __launch_bounds__(1024)
-    distillation_long_kernel(const T *z, RowMap zm, const acc_t<T> *top, const I *index, int k, int64_t vocab, acc_t<T> temp,
-                             acc_t<T> inv_temp, acc_t<T> *loss, acc_t<T> *stats)
-{
-    using A = acc_t<T>;
-    extern __shared__ __align__(16) char shared_bytes[];
-    __shared__ A buf[3][32];
-    __shared__ int used;
-    const uint32_t r = blockIdx.x;
-    const Teacher<A> teacher(shared_bytes, k);
-    if (threadIdx.x < 32) {
-        const bool any = teacher.read(top + int64_t(r) * k, index + int64_t(r) * k, k, vocab);
-        if (any) teacher.normalize(k, inv_temp);
-        if (threadIdx.x == 0) used = any;
-    }
-    __syncthreads();
-    if (!used) {
-        if (threadIdx.x == 0) {
-            if (loss) loss[r] = 0;
-            if (stats) stats[2 * int64_t(r)] = stats[2 * int64_t(r) + 1] = 0;
-        }
-        return;
-    }
-    const T *row = z + zm(r);
-    A best = -INFINITY;
-    for (int64_t c = threadIdx.x; c < vocab; c += blockDim.x) best = max_nan(best, to_acc<A>(row[c]));
-    best = block_fold(MaxNanF(), best, buf[0]);
-    A sum = 0;
-    for (int64_t c = threadIdx.x; c < vocab; c += blockDim.x)
-        sum += exp_((to_acc<A>(row[c]) - SoftSum<A>::finite(best)) * inv_temp);
-    sum = block_fold(SumF(), sum, buf[1]);
-    const A log_sum = log_(sum);
-    A s = 0;
-    for (int i = threadIdx.x; i < k; i += blockDim.x) {
-        if (teacher.at[i] < 0 || teacher.p[i] == 0) continue;
-        const A v = to_acc<A>(row[teacher.at[i]]);
-        s += teacher.p[i] * (teacher.logp[i] - (v == -INFINITY ? A(-INFINITY) : (v - best) * inv_temp - log_sum));
-    }
-    s = block_fold(SumF(), s, buf[2]);
-    if (threadIdx.x == 0) {
-        if (loss) loss[r] = temp * temp * s;
-        if (stats) {
-            stats[2 * int64_t(r)] = best;
-            stats[2 * int64_t(r) + 1] = log_sum;
-        }
-    }
+    part.teacher_gradient(out, grad);
 }
 
 // --------------------------------------------------------------------------------------- launchers
@@ -489,74 +464,67 @@ struct DistilArgs {
     double temp;
 };
 
-template <class T, class I> static int run_grad(const DistilArgs &a, const acc_t<T> *stats, cudaStream_t s)
+// Blocks that share a row: parts of `part` bytes at most, at most 2^most of them; few rows are split further, down to 8
+// KiB.
+static int share_row(const DistilArgs &a, int item, int64_t part, int most, Shares &share)
+{
+    const int64_t bytes = a.vocab * item, vec = 16 / item;
+    share.bits = 0;
+    while (share.bits < most && (bytes >> share.bits) > part) ++share.bits;
+    while (share.bits < most && (a.rows << share.bits) < 4 * device_props().sm_count && (bytes >> share.bits) >= 16 * 1024) ++share.bits;
+    if ((a.rows << share.bits) > INT32_MAX) return set_error(DPB_ERR_VALUE, "too many rows of this length");
+    share.each = static_cast<int>(ceil_div(a.vocab / vec, int64_t(1) << share.bits));
+    return DPB_OK;
+}
+
+// Threads of a block: up to two rounds of kInFlight accesses each before the block grows (short rows gain from more
+// blocks on an SM: 8192 x 5000 float16 takes 80 us with 256 threads, 49 with 128), at least two warps.
+static unsigned share_threads(const Shares &share)
+{
+    unsigned threads = 64;
+    while (threads < unsigned(kThreads) && share.each > 2 * kInFlight * static_cast<int>(threads)) threads *= 2;
+    return threads;
+}
+
+template <class T, class I> static int run_grad(const DistilArgs &a, cudaStream_t s)
 {
     using A = acc_t<T>;
-    // a part of 64 KiB a block amortises the teacher's entries; few rows are split further
-    const int64_t bytes = a.vocab * int64_t(sizeof(T));
-    int64_t ranks = std::max<int64_t>(1, bytes / (64 * 1024));
-    while (a.rows * ranks < 4 * device_props().sm_count && bytes / (2 * ranks) >= 8 * 1024) ranks *= 2;
-    ranks = std::min<int64_t>(ranks, INT32_MAX / a.rows);
-    launch_shared(distillation_grad_kernel<T, I>, static_cast<unsigned>(a.rows * ranks), unsigned(kThreads),
-                  (Teacher<A>::bytes(int(a.k)) + 15) / 16 * 16 + size_t(a.k) * sizeof(A), s, static_cast<const A *>(a.dloss->data),
-                  a.dloss->nd == 0 ? 0 : 1, static_cast<const T *>(a.z->data), a.zm, static_cast<const A *>(a.top->data),
-                  static_cast<const I *>(a.index->data), static_cast<int>(a.k), a.vocab, A(a.temp), A(1.0 / a.temp),
-                  A(kLog2E / a.temp), stats, static_cast<T *>(a.dz->data), a.dm, static_cast<int>(ranks));
+    Shares share;
+    // parts of 64 to 128 KiB: below that the teacher's entries, which every block reads, show (1024 x 150001 float32:
+    // 221 us at 75 KiB, 266 us at 37 KiB)
+    DPB_TRY(share_row(a, sizeof(T), 128 * 1024, 10, share));
+    launch_shared(distillation_grad_kernel<T, I>, static_cast<unsigned>(a.rows << share.bits), share_threads(share),
+                  RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const A *>(a.dloss->data), a.dloss->nd == 0 ? 0 : 1,
+                  static_cast<const T *>(a.z->data), a.zm, static_cast<const A *>(a.top->data),
+                  static_cast<const I *>(a.index->data), static_cast<int>(a.k), static_cast<int>(a.vocab), A(a.temp),
+                  A(1.0 / a.temp), A(kLog2E / a.temp), static_cast<const A *>(a.stats->data), static_cast<T *>(a.dz->data), a.dm, share);
     note_kernel("distillation_grad");
     return check_launch("distillation_grad");
 }
 
-template <class T, class I, bool GRAD> static int run_rows(const DistilArgs &a, int ranks, cudaStream_t s)
+template <class T, class I, bool GRAD> static int run_rows(const DistilArgs &a, cudaStream_t s)
 {
     using A = acc_t<T>;
-    constexpr int VEC = vec_width<T>();
-    const int64_t accesses = ceil_div(a.vocab / VEC, ranks);
-    int threads = 64;   // eight accesses a thread
-    while (threads < 512 && accesses > 8 * threads) threads *= 2;
-    const size_t shared = (Teacher<A>::bytes(int(a.k)) + 15) / 16 * 16 + size_t(accesses) * 16 + size_t(a.k) * sizeof(A);
-    launch_cluster(distillation_row_kernel<T, I, GRAD>, static_cast<unsigned>(a.rows * ranks), unsigned(ranks), unsigned(threads), shared, s,
-                   static_cast<const T *>(a.z->data), a.zm, static_cast<const A *>(a.top->data),
-                   static_cast<const I *>(a.index->data), static_cast<int>(a.k), a.vocab, A(a.temp), A(1.0 / a.temp),
-                   A(kLog2E / a.temp), a.loss ? static_cast<A *>(a.loss->data) : nullptr,
-                   a.stats ? static_cast<A *>(a.stats->data) : nullptr, GRAD ? static_cast<const A *>(a.dloss->data) : nullptr,
-                   GRAD && a.dloss->nd > 0 ? 1 : 0, GRAD ? static_cast<T *>(a.dz->data) : nullptr, a.dm, ranks);
+    Shares share;
+    // 4096 x 128000 float16: loss 186 us with whole rows of 250 KiB, 195 with halves, 238 with quarters; loss and
+    // gradient 421 with quarters, 477 with halves (what the clusters hold has to stay in the cache between the
+    // two readings)
+    DPB_TRY(share_row(a, sizeof(T), (GRAD ? 64 : 256) * 1024, 3, share));
+    launch_cluster(distillation_row_kernel<T, I, GRAD>, static_cast<unsigned>(a.rows << share.bits), 1u << share.bits, share_threads(share),
+                   RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const T *>(a.z->data), a.zm,
+                   static_cast<const A *>(a.top->data), static_cast<const I *>(a.index->data), static_cast<int>(a.k),
+                   static_cast<int>(a.vocab), A(a.temp), A(1.0 / a.temp), A(kLog2E / a.temp),
+                   a.loss ? static_cast<A *>(a.loss->data) : nullptr, a.stats ? static_cast<A *>(a.stats->data) : nullptr,
+                   GRAD ? static_cast<const A *>(a.dloss->data) : nullptr, GRAD && a.dloss->nd > 0 ? 1 : 0,
+                   GRAD ? static_cast<T *>(a.dz->data) : nullptr, a.dm, share);
     note_kernel("distillation_row");
     return check_launch("distillation_row");
 }
 
-template <class T, class I> static int run_long(const DistilArgs &a, acc_t<T> *stats, cudaStream_t s)
-{
-    using A = acc_t<T>;
-    distillation_long_kernel<T, I><<<static_cast<unsigned>(a.rows), 1024, Teacher<A>::bytes(int(a.k)), s>>>(
-        static_cast<const T *>(a.z->data), a.zm, static_cast<const A *>(a.top->data), static_cast<const I *>(a.index->data),
-        static_cast<int>(a.k), a.vocab, A(a.temp), A(1.0 / a.temp), a.loss ? static_cast<A *>(a.loss->data) : nullptr, stats);
-    note_kernel("distillation_long");
-    return check_launch("distillation_long");
-}
-
-// Blocks that share a row so that each holds at most 64 KiB (three blocks an SM are in different phases then); few
-// rows are spread over more blocks as long as each has 8 KiB.  0: more than 8 blocks of 200 KiB.
-static int row_ranks(int64_t rows, int64_t bytes)
-{
-    int ranks = 1;
-    while (ranks < kMaxRanks && bytes > int64_t(ranks) * 64 * 1024) ranks *= 2;
-    while (ranks < kMaxRanks && rows * ranks < 2 * device_props().sm_count && bytes / (2 * ranks) >= 8 * 1024) ranks *= 2;
-    return bytes <= int64_t(ranks) * 200 * 1024 && rows <= INT32_MAX / ranks ? ranks : 0;
-}
-
 template <class T, class I> static int run(const DistilArgs &a, cudaStream_t s)
 {
-    using A = acc_t<T>;
-    if (a.dz && !a.loss) return run_grad<T, I>(a, static_cast<const A *>(a.stats->data), s);
-    const int ranks = row_ranks(a.rows, a.vocab * int64_t(sizeof(T)));
-    if (ranks > 0) return a.dz ? run_rows<T, I, true>(a, ranks, s) : run_rows<T, I, false>(a, ranks, s);
-    if (!a.dz) return run_long<T, I>(a, a.stats ? static_cast<A *>(a.stats->data) : nullptr, s);
-    void *work = nullptr;
-    DPB_TRY(dpb_malloc(static_cast<size_t>(2 * a.rows) * sizeof(A), s, &work));
-    int st = run_long<T, I>(a, static_cast<A *>(work), s);
-    if (st == DPB_OK) st = run_grad<T, I>(a, static_cast<const A *>(work), s);
-    dpb_free(work, s);
-    return st;
+    if (a.dz && !a.loss) return run_grad<T, I>(a, s);
+    return a.dz ? run_rows<T, I, true>(a, s) : run_rows<T, I, false>(a, s);
 }
 
 static int run_typed(const DistilArgs &a, cudaStream_t s)

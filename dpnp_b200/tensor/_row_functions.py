@@ -151,6 +151,127 @@ def _unpack_out(out, count, what):
     return tuple(out)
 
 
+# ------------------------------------------------------------------------------------------- direct route
+# A call whose arrays are C-contiguous and live on one queue object goes to the library as it is: the types and
+# shapes that results are allocated from are compared here, everything else is checked by the library, and
+# whatever it refuses takes the general route below, which copies what has to be copied and words the refusal.
+# (As for the elementwise functions, the general route is the specification.)
+_nat = tri._nat
+_new = usm_ndarray._new_dense
+
+
+def _plain(q, *arrays):
+    """Whether all arrays (None: absent) are C-contiguous and on the queue `q`."""
+    for a in arrays:
+        if a is not None and (type(a) is not usm_ndarray or a._queue is not q or not a._flags & _lib.FLAG_C):
+            return False
+    return True
+
+
+def _plain_rows(q, *arrays):
+    """The same for arrays of rows, which may lie apart."""
+    for a in arrays:
+        if a is not None and (type(a) is not usm_ndarray or a._queue is not q
+                              or not (a._flags & _lib.FLAG_C or _walkable(a._shape, a._strides))):
+            return False
+    return True
+
+
+def _core(a):
+    return None if a is None else a._core()
+
+
+def _outs(out, count):
+    """`out` of an operator with `count` results as that many entries; None when it is something else."""
+    if out is None:
+        return (None,) * count
+    if count == 1:
+        return (out,)
+    return out if type(out) is tuple and len(out) == count else None
+
+
+def _weights_fit(x, *weights):
+    """Weights of the last axis, all of one type that goes with x."""
+    dt = None
+    for w in weights:
+        if w is None:
+            continue
+        if w._shape != x._shape[-1:] or (dt is not None and w._dtype != dt):
+            return False
+        dt = w._dtype
+    return dt is None or dt == x._dtype or (dt == _SINGLE and x._dtype == _HALF)
+
+
+def _direct_layer_norm(x, weight, bias, eps, return_stats, out):
+    outs = _outs(out, 3 if return_stats else 1)
+    if outs is None or type(x) is not usm_ndarray or type(eps) is not float or not 0 <= eps < float("inf") or not x._shape:
+        return None
+    q, acc = x._queue, _ACCUMULATION.get(x._dtype)
+    if acc is None or x._shape[-1] == 0 or not _plain_rows(q, x, outs[0]) or not _plain(q, weight, bias, *outs[1:]) \
+            or not _weights_fit(x, weight, bias):
+        return None
+    y = _new(x._shape, x._dtype, q) if outs[0] is None else outs[0]
+    mean = rstd = None
+    if return_stats:
+        lead = x._shape[:-1]
+        mean = _new(lead, acc, q) if outs[1] is None else outs[1]
+        rstd = _new(lead, acc, q) if outs[2] is None else outs[2]
+    try:
+        _nat.layer_norm(x._core(), _core(weight), _core(bias), eps, y._core(), _core(mean), _core(rstd), q._stream)
+    except (TypeError, ValueError):
+        return None
+    return (y, mean, rstd) if return_stats else y
+
+
+def _direct_layer_norm_backward(dy, x, mean, rstd, weight, weight_grads, out):
+    outs = _outs(out, 3)
+    if outs is None or type(x) is not usm_ndarray or not x._shape or not weight_grads:
+        return None
+    q = x._queue
+    if not _plain_rows(q, x, dy, outs[0]) or not _plain(q, mean, rstd, weight, *outs[1:]) or x._dtype not in _ACCUMULATION or x._shape[-1] == 0:
+        return None
+    if dy._shape != x._shape or dy._dtype != x._dtype or mean._shape != x._shape[:-1] or not _weights_fit(x, weight):
+        return None
+    dx, dw, db = outs
+    if weight is None and (dw is not None or db is not None):
+        return None
+    wt = x._dtype if weight is None else weight._dtype
+    dx = _new(x._shape, x._dtype, q) if dx is None else dx
+    dw = _new(x._shape[-1:], wt, q) if dw is None else dw
+    db = _new(x._shape[-1:], wt, q) if db is None else db
+    try:
+        _nat.layer_norm_backward(dy._core(), x._core(), mean._core(), rstd._core(), _core(weight), dx._core(), dw._core(),
+                                 db._core(), q._stream)
+    except (TypeError, ValueError):
+        return None
+    return dx, dw, db
+
+
+def _direct_embedding(table, ids, scale, out):
+    if type(table) is not usm_ndarray or type(ids) is not usm_ndarray or type(scale) is not float or len(table._shape) != 2:
+        return None
+    q = table._queue
+    if not _plain(q, ids) or not _plain_rows(q, table, out) or ids._dtype not in _INDEX or table._dtype not in _ACCUMULATION:
+        return None
+    out = _new(ids._shape + table._shape[1:], table._dtype, q) if out is None else out
+    try:
+        _nat.embedding(table._core(), ids._core(), scale, out._core(), q._stream)
+    except (TypeError, ValueError):
+        return None
+    return out
+
+
+def _direct_distillation(logits, teacher_logits, teacher_index, temperature):
+    """Whether the inputs of a distillation are ready for the library."""
+    if type(logits) is not usm_ndarray or type(temperature) is not float:
+        return False
+    acc = _ACCUMULATION.get(logits._dtype)
+    return (acc is not None and _plain_rows(logits._queue, logits) and _plain(logits._queue, teacher_logits, teacher_index)
+            and teacher_logits is not None and teacher_index is not None and teacher_logits._dtype == acc
+            and teacher_index._dtype in _INDEX and len(logits._shape) > 0
+            and teacher_logits._shape[:-1] == logits._shape[:-1] and teacher_index._shape == teacher_logits._shape)
+
+
 # ------------------------------------------------------------------------------------ layer normalisation
 class _Normalized:
     """The axes of a layer normalisation: the kernel sees the remaining axes, then one axis with all of the
@@ -251,6 +372,10 @@ def layer_norm(x, weight=None, bias=None, /, *, axis=-1, eps=1e-5, return_stats=
     out : array for the result, or with `return_stats` a tuple of three (None: allocated).  The result may
         be written over `x`.
     """
+    if axis == -1 and _nat is not None:
+        res = _direct_layer_norm(x, weight, bias, eps, return_stats, out)
+        if res is not None:
+            return res
     _check_array(x, "x")
     for w, what in ((weight, "weight"), (bias, "bias")):
         if w is not None:
@@ -290,6 +415,10 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, /, *, axis=-1, weight_gr
 
     The sums over the rows have a fixed order: the same call gives the same bits.
     """
+    if axis == -1 and _nat is not None:
+        res = _direct_layer_norm_backward(dy, x, mean, rstd, weight, weight_grads, out)
+        if res is not None:
+            return res
     for a, what in ((dy, "dy"), (x, "x"), (mean, "mean"), (rstd, "rstd")):
         _check_array(a, what)
     if weight is not None:
@@ -343,6 +472,10 @@ def embedding(table, ids, /, *, scale=1.0, out=None):
         names no row: its result is a row of zeros.  (uint64 ids of 2**63 and above are outside, too.)
     out : array of shape ``ids.shape + table.shape[1:]`` and the type of `table`.
     """
+    if _nat is not None:
+        res = _direct_embedding(table, ids, scale, out)
+        if res is not None:
+            return res
     _check_array(table, "table")
     _check_ids(ids)
     _accumulation_type(table, "table")
@@ -443,8 +576,21 @@ def distillation_loss(logits, teacher_logits, teacher_index, /, *, temperature=1
     out : array for the losses, or with `return_stats` a tuple of two (None: allocated).
 
     Loss and statistics are float32, or float64 for float64 logits.  Where q is 0 and p is not (a student
-    logit of -inf at the teacher's column) the loss is +inf; NaN and +inf in a row that counts give NaN.
+    logit of -inf at the teacher's column) the loss is +inf; NaN and +inf in a row that counts make its loss and
+    its gradient NaN.
     """
+    if _nat is not None and _direct_distillation(logits, teacher_logits, teacher_index, temperature):
+        outs, q = _outs(out, 2 if return_stats else 1), logits._queue
+        if outs is not None and _plain(q, *outs):
+            acc, lead = teacher_logits._dtype, logits._shape[:-1]
+            loss = _new(lead, acc, q) if outs[0] is None else outs[0]
+            stats = None if not return_stats else _new(lead + (2,), acc, q) if outs[1] is None else outs[1]
+            try:
+                _nat.distillation_loss(logits._core(), teacher_logits._core(), teacher_index._core(), temperature,
+                                       loss._core(), _core(stats), q._stream)
+                return (loss, stats) if return_stats else loss
+            except (TypeError, ValueError):
+                pass
     acc, temperature = _distillation_args(logits, teacher_logits, teacher_index, temperature)
     q = _execution_queue(logits, teacher_logits, teacher_index)
     if return_stats:
@@ -470,6 +616,16 @@ def distillation_loss_backward(dloss, logits, teacher_logits, teacher_index, sta
     stats : the statistics that ``distillation_loss(..., return_stats=True)`` returned for these logits.
     out : array of the shape and type of `logits`; the result may be written over `logits`.
     """
+    if _nat is not None and _direct_distillation(logits, teacher_logits, teacher_index, temperature):
+        q = logits._queue
+        if type(dloss) is usm_ndarray and stats is not None and _plain(q, dloss, stats) and _plain_rows(q, out):
+            dz = _new(logits._shape, logits._dtype, q) if out is None else out
+            try:
+                _nat.distillation_loss_backward(dloss._core(), logits._core(), teacher_logits._core(), teacher_index._core(),
+                                                stats._core(), temperature, dz._core(), q._stream)
+                return dz
+            except (TypeError, ValueError):
+                pass
     acc, temperature = _distillation_args(logits, teacher_logits, teacher_index, temperature)
     _check_array(stats, "stats")
     lead = logits._shape[:-1]
@@ -496,6 +652,17 @@ def distillation_loss_and_grad(logits, teacher_logits, teacher_index, dloss=1.0,
 
     out : tuple of two arrays (None: allocated); the gradient may be written over `logits`.
     """
+    if _nat is not None and _direct_distillation(logits, teacher_logits, teacher_index, temperature):
+        outs, q = _outs(out, 2), logits._queue
+        if outs is not None and type(dloss) is usm_ndarray and _plain(q, dloss, outs[0]) and _plain_rows(q, outs[1]):
+            loss = _new(logits._shape[:-1], teacher_logits._dtype, q) if outs[0] is None else outs[0]
+            dz = _new(logits._shape, logits._dtype, q) if outs[1] is None else outs[1]
+            try:
+                _nat.distillation_loss_and_grad(logits._core(), teacher_logits._core(), teacher_index._core(), dloss._core(),
+                                                temperature, loss._core(), dz._core(), q._stream)
+                return loss, dz
+            except (TypeError, ValueError):
+                pass
     acc, temperature = _distillation_args(logits, teacher_logits, teacher_index, temperature)
     lead = logits._shape[:-1]
     given = dloss if isinstance(dloss, usm_ndarray) else None
