@@ -124,6 +124,35 @@ def test_layer_norm_many_rows(dt, wt):
         check_norm(x, w, b, 1e-5, host(y), host(mean), host(rstd))
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,n,pad", [(2, 37, 1), (9, 37, 0), (1183, 37, 0), (1200, 300, 5), (2500, 301, 1), (1300, 2049, 0),
+                                        (297, 4095, 2), (600, 8191, 1), (593, 130, 0), (1000, 5, 3)])
+def test_layer_norm_rows_off_the_vector_grid(dt, rows, n, pad):
+    """Odd widths and padded rows, row counts around the numbers of blocks; x, dy and the results start at different
+    places within 16 bytes."""
+    import dpnp_b200 as dp
+
+    if rows * n > 2e6 and dt == "f8":
+        rows //= 3
+    x, w, b, rng = norm_data(rows, n + pad, dt, dt, rows + n)
+    w, b, dy = w[:n], b[:n], rng.normal(0, 1, (rows, n)).astype(dt)
+    d = dev(x)[:, pad // 2:pad // 2 + n]
+    x = np.ascontiguousarray(x[:, pad // 2:pad // 2 + n])
+    y, mean, rstd = dp.layer_norm(d, dev(w), dev(b), return_stats=True)
+    check_norm(x, w, b, 1e-5, host(y), host(mean), host(rstd))
+    out = dp.layer_norm_backward(dev(dy), d, mean, rstd, dev(w))
+    check_norm_backward(x, dy, w, host(mean), host(rstd), *map(host, out))
+    buf = dp.zeros(rows * n + 8, dtype=dt)
+    shifted = buf[3:rows * n + 3].reshape(rows, n)
+    shifted[:] = dev(dy)
+    out = dp.layer_norm_backward(shifted, d, mean, rstd, dev(w))
+    check_norm_backward(x, dy, w, host(mean), host(rstd), *map(host, out))
+    target = buf[1:rows * n + 1].reshape(rows, n)
+    dp.layer_norm(d, dev(w), dev(b), out=target)
+    check_norm(x, w, b, 1e-5, host(target), host(mean), host(rstd))
+    assert not host(buf)[:1].any() and not host(buf)[rows * n + 4:].any()
+
+
 def check_norm_backward(x, dy, w, mean, rstd, dx, dw, db):
     dt = x.dtype.str[1:]
     wide, u, n = WIDE[dt], unit(dt), x.shape[-1]
@@ -425,6 +454,24 @@ def test_embedding_backward_distributions(kind):
     check_embedding_backward(dout, ids, rows, 1.0, got, "f4")
 
 
+@pytest.mark.parametrize("tokens,rows,n,idt", [(140000, 1000, 24, "i4"), (70000, 300000, 4, "i8"), (1500, 600000, 3, "i4"),
+                                               (131073, 5, 8, "i8"), (90000, 40, 2050, "i4")])
+def test_embedding_backward_long_batches(tokens, rows, n, idt):
+    """Several tiles of the sort and more than the tiles that are placed without a scan; tables of one to three digits;
+    long chunks, and ids that span hundreds of them."""
+    import dpnp_b200 as dp
+
+    rng = np.random.default_rng(tokens)
+    ids = (rows * rng.uniform(0, 1, tokens)**4).astype(idt)
+    ids[rng.uniform(0, 1, tokens) < 0.3] = rows // 2
+    ids[rng.uniform(0, 1, tokens) < 0.02] = -7
+    dout = rng.normal(0, 1, (tokens, n)).astype("f4" if n > 1000 else "f8")
+    got = dp.embedding_backward(dev(dout), dev(ids), rows, scale=2.0)
+    check_embedding_backward(dout, ids, rows, 2.0, host(got), dout.dtype.str[1:])
+    again = dp.embedding_backward(dev(dout), dev(ids), rows, scale=2.0)
+    assert np.array_equal(host(again), host(got))
+
+
 def test_embedding_backward_layouts():
     import dpnp_b200 as dp
 
@@ -714,6 +761,28 @@ def _step(dp, a):
 RESULTS = ("x", "y", "mean", "rstd", "loss", "stats", "dy", "loss2", "dy2", "dx", "dw", "db", "dtable")
 
 
+@pytest.mark.parametrize("sizes", [dict(tokens=3, vocab=50, n=40001, k=70), dict(tokens=2100, vocab=3000, n=64, k=3)])
+def test_captured_passes_of_other_shapes(sizes):
+    """Rows shared by clusters of blocks, and a sort of several tiles, captured and replayed."""
+    torch = pytest.importorskip("torch")
+    import dpnp_b200 as dp
+
+    tensors = _tensors(torch, 9, **sizes)
+    torch.cuda.synchronize()
+    _step(dp, _arrays(dp, tensors, dp.StreamQueue(0, stream=torch.cuda.current_stream().cuda_stream)))
+    torch.cuda.synchronize()
+    want = {k: tensors[k].clone() for k in RESULTS}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _step(dp, _views(dp, tensors, dp.StreamQueue(0, stream=torch.cuda.current_stream().cuda_stream)))
+    for k in RESULTS:
+        tensors[k].zero_()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(tensors[k], want[k]) for k in RESULTS)
+
+
 def _tensors(torch, seed, tokens=700, vocab=900, n=1031, k=5):
     gen = torch.Generator(device="cuda").manual_seed(seed)
     f = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
@@ -726,6 +795,12 @@ def _tensors(torch, seed, tokens=700, vocab=900, n=1031, k=5):
 
 def _arrays(dp, tensors, queue):
     return {k: dp.from_dlpack(v, device=queue) for k, v in tensors.items()}
+
+
+def _views(dp, tensors, queue):
+    """The same without the exchange's synchronisation, which a capture does not allow."""
+    return {k: dp.tensor.usm_ndarray._view(None, v.data_ptr(), tuple(v.shape), tuple(v.stride()),
+                                           np.dtype(str(v.dtype).split(".")[1]), queue) for k, v in tensors.items()}
 
 
 def test_two_captured_passes_replayed_side_by_side():
@@ -747,9 +822,7 @@ def test_two_captured_passes_replayed_side_by_side():
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
             queue = dp.StreamQueue(0, stream=torch.cuda.current_stream().cuda_stream)
-            arrays = {k: dp.tensor.usm_ndarray._view(None, v.data_ptr(), tuple(v.shape), tuple(v.stride()),
-                                                     np.dtype(str(v.dtype).split(".")[1]), queue) for k, v in tensors.items()}
-            _step(dp, arrays)
+            _step(dp, _views(dp, tensors, queue))
         graphs.append(graph)
         streams.append(stream)
     for _ in range(3):
