@@ -37,13 +37,49 @@ struct RowSequence {
     }
 };
 
+// Access k of a row that starts `mis` elements behind a 16-byte boundary begins at column k VEC - mis: all but the
+// first and the last are whole and aligned.  A row of n elements has at most n + VEC - 1 over VEC of them (rounded up).
+template <class T, int VEC> struct ShiftedColumn {
+    int64_t c;
+    int64_t n;
+    DPB_D ShiftedColumn(const T *row, uint32_t k, int64_t n_) : c(int64_t(k) * VEC - misalignment_of(row)), n(n_) {}
+    static DPB_D int misalignment_of(const T *row)
+    {
+        return static_cast<int>(reinterpret_cast<uintptr_t>(row) % (VEC * sizeof(T))) / static_cast<int>(sizeof(T));
+    }
+    DPB_D bool whole() const { return c >= 0 && c + VEC <= n; }
+    DPB_D bool has(int j) const { return c + j >= 0 && c + j < n; }
+    // from a row that may start anywhere; zeros outside it
+    template <class S> DPB_D vec_t<S, VEC> load(const S *row, const Span<S> &array) const
+    {
+        if (whole()) {
+            if constexpr (VEC * sizeof(S) == 16) return load_anywhere<S, VEC>(row + c, array.lo, array.hi);
+        }
+        vec_t<S, VEC> v;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v.v[j] = has(j) ? row[c + j] : from_acc<S>(acc_t<S>(0));
+        return v;
+    }
+    DPB_D void store(T *row, const vec_t<T, VEC> &v) const
+    {
+        if (whole()) *reinterpret_cast<vec_t<T, VEC> *>(row + c) = v;
+        else
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (has(j)) row[c + j] = v.v[j];
+    }
+};
+
 // ----------------------------------------------------------------------------------------- forward
-// A copy with a gather: bound by memory, so four accesses of VEC elements in flight a thread.
-template <class T, class I, int VEC>
-__global__ void __launch_bounds__(kThreads) embedding_kernel(const T *table, int64_t ld, const I *ids, acc_t<T> scale, T *out,
-                                                             RowMap om, int64_t vocab, int64_t tokens, RowSequence seq)
+// A copy with a gather: bound by memory, so four accesses in flight a thread.  SHIFT: rows start anywhere; the stores
+// are aligned, the loads shifted into place.
+template <class T, class I, bool SHIFT>
+__global__ void __launch_bounds__(kThreads) embedding_kernel(const T *table, int64_t ld, Span<T> array, const I *ids, acc_t<T> scale,
+                                                             T *out, RowMap om, int64_t vocab, int64_t tokens, int64_t n,
+                                                             RowSequence seq)
 {
     using A = acc_t<T>;
+    constexpr int VEC = vec_width<T>();
     using V = vec_t<T, VEC>;
     cudaGridDependencySynchronize();
     int64_t row;
@@ -60,8 +96,13 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const T *table, int
     }
     V v[kAccesses];
 #pragma unroll
-    for (int k = 0; k < kAccesses; ++k)
-        if (id[k] >= 0 && id[k] < vocab) v[k] = load_vec<V>(table + id[k] * ld + int64_t(c[k]) * VEC);
+    for (int k = 0; k < kAccesses; ++k) {
+        if (id[k] < 0 || id[k] >= vocab) continue;
+        const T *from = table + id[k] * ld;
+        if constexpr (SHIFT)
+            v[k] = ShiftedColumn<T, VEC>(out + om(static_cast<uint32_t>(token[k])), c[k], n).load(from, array);
+        else v[k] = load_vec<V>(from + int64_t(c[k]) * VEC);
+    }
 #pragma unroll
     for (int k = 0; k < kAccesses; ++k) {
         if (token[k] >= tokens) continue;
@@ -71,7 +112,10 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const T *table, int
             unpack<A, VEC, T>(v[k], u);
             u.mul(scale);
         }
-        *reinterpret_cast<V *>(out + om(static_cast<uint32_t>(token[k])) + int64_t(c[k]) * VEC) = repack<T, VEC, A>(u);
+        T *to = out + om(static_cast<uint32_t>(token[k]));
+        const V w = repack<T, VEC, A>(u);
+        if constexpr (SHIFT) ShiftedColumn<T, VEC>(to, c[k], n).store(to, w);
+        else *reinterpret_cast<V *>(to + int64_t(c[k]) * VEC) = w;
     }
 }
 
@@ -92,9 +136,10 @@ constexpr int kJoinedTiles = 64;
 // begin with the gradient's zeros (of rows that occur, too: they are written again later).
 struct ZeroRows {
     char *base;
-    int64_t row_bytes;   // from one row to the next
-    int access;          // bytes: 16, 8, 4 or 2
-    RowSequence seq;
+    int64_t row_bytes;     // from one row to the next
+    int64_t bytes;         // of a row
+    int item;              // bytes of an element
+    RowSequence seq;       // accesses of 16 bytes, shifted to the rows' starts
     int64_t rows, first;   // first access of this launch
     int64_t blocks;
 };
@@ -108,11 +153,15 @@ DPB_D void zero_rows(const ZeroRows &z, int64_t block)
         uint32_t q, c;
         z.seq.per_row.divmod(rest + k * kThreads + threadIdx.x, q, c);
         if (row + q >= z.rows) continue;
-        char *p = z.base + (row + q) * z.row_bytes + int64_t(c) * z.access;
-        if (z.access == 16) *reinterpret_cast<int4 *>(p) = make_int4(0, 0, 0, 0);
-        else if (z.access == 8) *reinterpret_cast<int2 *>(p) = make_int2(0, 0);
-        else if (z.access == 4) *reinterpret_cast<int *>(p) = 0;
-        else *reinterpret_cast<short *>(p) = 0;
+        char *start = z.base + (row + q) * z.row_bytes;
+        const int64_t at = int64_t(c) * 16 - int64_t(reinterpret_cast<uintptr_t>(start) % 16);
+        if (at >= 0 && at + 16 <= z.bytes) *reinterpret_cast<int4 *>(start + at) = make_int4(0, 0, 0, 0);
+        else
+            for (int64_t i = max(at, int64_t(0)); i < min(at + 16, z.bytes); i += z.item) {
+                if (z.item == 2) *reinterpret_cast<short *>(start + i) = 0;
+                else if (z.item == 4) *reinterpret_cast<int *>(start + i) = 0;
+                else *reinterpret_cast<long long *>(start + i) = 0;
+            }
     }
 }
 
@@ -389,17 +438,24 @@ constexpr int kInFlight = 8;    // rows' loads of a thread in flight
 // of one that starts here and goes on.  The other blocks write the rows that do not occur (from access `zeroed`
 // on), kAccesses accesses a thread.  Every `stride`-th block is one of the first kind: reads and writes
 // overlap.
-template <class T, class O, int VEC>
-__global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout, RowMap dm, const uint32_t *key, const uint32_t *pos,
-                                                                  uint32_t tokens, const uint8_t *mark, acc_t<T> *part,
-                                                                  acc_t<T> scale, O *dtable, int64_t ld, uint32_t vocab,
-                                                                  RowSequence seq, uint32_t sum_blocks, FastDiv32 tiles,
-                                                                  FastDiv32 stride, int64_t zeroed, uint32_t chunk)
+template <class T, class O, bool SHIFT>
+__global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout, RowMap dm, Span<T> array, const uint32_t *key,
+                                                                  const uint32_t *pos, uint32_t tokens, const uint8_t *mark,
+                                                                  acc_t<T> *part, acc_t<T> scale, O *dtable, int64_t ld,
+                                                                  uint32_t vocab, int64_t n, RowSequence seq, uint32_t sum_blocks,
+                                                                  FastDiv32 tiles, FastDiv32 stride, int64_t zeroed, uint32_t chunk)
 {
     using A = acc_t<T>;
+    constexpr int VEC = vec_width<T>(), flight = SHIFT ? kInFlight / 2 : kInFlight;
     using V = vec_t<T, VEC>;
     using VO = vec_t<O, VEC>;
     using Vals = Values<A, VEC>;
+    const auto write = [&](int64_t v, uint32_t c, const Vals &s) {
+        const VO w = repack<O, VEC, A>(s);
+        O *to = dtable + v * ld;
+        if constexpr (SHIFT) ShiftedColumn<O, VEC>(to, c, n).store(to, w);
+        else *reinterpret_cast<VO *>(to + int64_t(c) * VEC) = w;
+    };
     cudaGridDependencySynchronize();
     uint32_t block, off;
     stride.divmod(blockIdx.x, block, off);
@@ -409,13 +465,12 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
         seq.start(zeroed + int64_t(blockIdx.x - min(block + (off != 0), sum_blocks)) * (kThreads * kAccesses), row, rest);
         Vals zero;
         zero.fill(0);
-        const VO z = repack<O, VEC, A>(zero);
 #pragma unroll
         for (int k = 0; k < kAccesses; ++k) {
             uint32_t q, c;
             seq.per_row.divmod(rest + k * kThreads + threadIdx.x, q, c);
             const int64_t v = row + q;
-            if (v < vocab && !mark[v]) *reinterpret_cast<VO *>(dtable + v * ld + int64_t(c) * VEC) = z;
+            if (v < vocab && !mark[v]) write(v, c, zero);
         }
         return;
     }
@@ -430,18 +485,22 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
     }
     if (threadIdx.x < count) rows[threadIdx.x] = dm(pos[begin + threadIdx.x]);
     __syncthreads();
-    const int64_t c = int64_t(tile) * kThreads + threadIdx.x;
+    const uint32_t c = tile * kThreads + threadIdx.x;
     if (c >= seq.per_row.d) return;
     Vals s, u;
     s.fill(0);
     bool whole = keys[0] != keys[1];   // the current run starts in this chunk
-    for (uint32_t i0 = 0; i0 < count; i0 += kInFlight) {
-        V v[kInFlight];
+    for (uint32_t i0 = 0; i0 < count; i0 += flight) {
+        V v[flight];
 #pragma unroll
-        for (int j = 0; j < kInFlight; ++j)
-            if (i0 + j < count && keys[i0 + j + 1] < vocab) v[j] = load_vec<V>(dout + rows[i0 + j] + c * VEC);
+        for (int j = 0; j < flight; ++j) {
+            if (i0 + j >= count || keys[i0 + j + 1] >= vocab) continue;
+            const T *from = dout + rows[i0 + j];
+            if constexpr (SHIFT) v[j] = ShiftedColumn<O, VEC>(dtable + int64_t(keys[i0 + j + 1]) * ld, c, n).load(from, array);
+            else v[j] = load_vec<V>(from + int64_t(c) * VEC);
+        }
 #pragma unroll
-        for (int j = 0; j < kInFlight; ++j) {
+        for (int j = 0; j < flight; ++j) {
             const uint32_t i = i0 + j;
             if (i >= count) break;
             const uint32_t id = keys[i + 1];
@@ -452,7 +511,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
             if (!ends && i + 1 < count) continue;
             if (whole && ends) {
                 s.mul(scale);
-                *reinterpret_cast<VO *>(dtable + id * ld + c * VEC) = repack<O, VEC, A>(s);
+                write(id, c, s);
             }
             else *reinterpret_cast<Vals *>(part + (int64_t(2 * k + whole) * seq.per_row.d + c) * VEC) = s;
             s.fill(0);
@@ -462,10 +521,10 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
 }
 
 // Runs over several chunks: the block of the chunk in which one ends adds its parts in order.
-template <class A, class O, int VEC>
+template <class A, class O, int VEC, bool SHIFT>
 __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t *key, uint32_t tokens, const A *part, A scale,
-                                                                  O *dtable, int64_t ld, uint32_t vocab, uint32_t per_row,
-                                                                  uint32_t chunk)
+                                                                  O *dtable, int64_t ld, uint32_t vocab, int64_t n,
+                                                                  uint32_t per_row, uint32_t chunk)
 {
     using Vals = Values<A, VEC>;
     cudaGridDependencySynchronize();
@@ -489,7 +548,10 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t
 #pragma unroll 8
     for (uint32_t g = first; g <= k; ++g) s.add(p[int64_t(2 * g) * per_row]);
     s.mul(scale);
-    *reinterpret_cast<vec_t<O, VEC> *>(dtable + id * ld + int64_t(c) * VEC) = repack<O, VEC, A>(s);
+    const vec_t<O, VEC> w = repack<O, VEC, A>(s);
+    O *to = dtable + id * ld;
+    if constexpr (SHIFT) ShiftedColumn<O, VEC>(to, c, n).store(to, w);
+    else *reinterpret_cast<vec_t<O, VEC> *>(to + int64_t(c) * VEC) = w;
 }
 
 // --------------------------------------------------------------------------------------- launchers
@@ -505,23 +567,36 @@ static unsigned sequence_blocks(int64_t rows, int64_t per_row)
     return static_cast<unsigned>(ceil_div(rows * per_row, kThreads * kAccesses));
 }
 
-template <class T, class I, int VEC> static void launch_forward(const EmbedArgs &a, cudaStream_t s)
+// Accesses of 16 bytes a row: without and with a shift to the row's start (two partial ones then).
+static int64_t row_accesses(int64_t n, int vec, bool shift)
 {
-    const int64_t per_row = a.n / VEC;
-    launch_after_previous(embedding_kernel<T, I, VEC>, sequence_blocks(a.tokens, per_row), unsigned(kThreads), s,
-                          static_cast<const T *>(a.table->data), a.ld, static_cast<const I *>(a.ids->data), acc_t<T>(a.scale),
-                          static_cast<T *>(a.out->data), a.om, a.vocab, a.tokens, RowSequence{FastDiv32(uint32_t(per_row))});
+    return shift ? ceil_div(n + vec - 1, vec) : n / vec;
 }
 
-// Accesses of 16 bytes where all rows allow them, else (float16) of 4 bytes, else single elements.
+template <class T> static Span<T> span_of(const dpb_array &a)
+{
+    const void *lo, *hi;
+    array_bounds(a, lo, hi);
+    return {static_cast<const T *>(lo), static_cast<const T *>(hi)};
+}
+
+template <class T, class I, bool SHIFT> static void launch_forward(const EmbedArgs &a, cudaStream_t s)
+{
+    const int64_t per_row = row_accesses(a.n, vec_width<T>(), SHIFT);
+    launch_after_previous(embedding_kernel<T, I, SHIFT>, sequence_blocks(a.tokens, per_row), unsigned(kThreads), s,
+                          static_cast<const T *>(a.table->data), a.ld, span_of<T>(*a.table), static_cast<const I *>(a.ids->data),
+                          acc_t<T>(a.scale), static_cast<T *>(a.out->data), a.om, a.vocab, a.tokens, a.n,
+                          RowSequence{FastDiv32(uint32_t(per_row))});
+}
+
 template <class T, class I> static int run_forward(const EmbedArgs &a, cudaStream_t s)
 {
     constexpr int wide = vec_width<T>();
     const RowMap table = {0, a.ld, FastDiv32(1)};
-    const int v = std::min(row_vector(a.out->data, a.om, a.n, sizeof(T), wide), row_vector(a.table->data, table, a.n, sizeof(T), wide));
-    if (v == wide) launch_forward<T, I, wide>(a, s);
-    else if (is_half_v<T> && v >= 2) launch_forward<T, I, is_half_v<T> ? 2 : 1>(a, s);
-    else launch_forward<T, I, 1>(a, s);
+    const bool aligned = row_vector(a.out->data, a.om, a.n, sizeof(T), wide) == wide &&
+                         row_vector(a.table->data, table, a.n, sizeof(T), wide) == wide;
+    if (aligned) launch_forward<T, I, false>(a, s);
+    else launch_forward<T, I, true>(a, s);
     note_kernel("embedding");
     return check_launch("embedding");
 }
@@ -540,7 +615,7 @@ static int64_t take_zeros(ZeroRows &z, int64_t bytes)
 {
     z.first += z.blocks * (kThreads * kAccesses);
     const int64_t left = std::max<int64_t>(0, z.rows * z.seq.per_row.d - z.first);
-    z.blocks = ceil_div(std::min(left, bytes / z.access), kThreads * kAccesses);
+    z.blocks = ceil_div(std::min(left, bytes / 16), kThreads * kAccesses);
     return z.blocks;
 }
 
@@ -605,29 +680,33 @@ struct EmbedGradArgs {
     double scale;
 };
 
-template <class T, class O, int VEC> static void run_sums(const EmbedGradArgs &a, void *work, size_t head, uint32_t chunk, cudaStream_t s)
+template <class T, class O, bool SHIFT>
+static void run_sums(const EmbedGradArgs &a, void *work, size_t head, uint32_t chunk, cudaStream_t s)
 {
     using A = acc_t<T>;
+    constexpr int VEC = vec_width<T>();
     uint32_t *w = static_cast<uint32_t *>(work), *key = nullptr, *pos = nullptr;
     uint8_t *mark = reinterpret_cast<uint8_t *>(w + sort_words(a.tokens));
     A *part = reinterpret_cast<A *>(static_cast<char *>(work) + head);
-    const int64_t per_row = a.n / VEC, tiles = ceil_div(per_row, kThreads), chunks = ceil_div(a.tokens, int64_t(chunk));
+    const int64_t per_row = row_accesses(a.n, VEC, SHIFT), tiles = ceil_div(per_row, kThreads), chunks = ceil_div(a.tokens, int64_t(chunk));
     O *dtable = static_cast<O *>(a.dtable->data);
-    // (a float32 gradient of float16 data takes two of these accesses for each of the sums')
-    constexpr int access = VEC * sizeof(O) > 16 ? 16 : VEC * static_cast<int>(sizeof(O));
-    ZeroRows zero = {reinterpret_cast<char *>(dtable), a.ld * int64_t(sizeof(O)), access,
-                     {FastDiv32(uint32_t(a.n * sizeof(O) / access))}, a.vocab, 0, 0};
+    const bool on_grid = !SHIFT && a.n * sizeof(O) % 16 == 0;
+    ZeroRows zero = {reinterpret_cast<char *>(dtable), a.ld * int64_t(sizeof(O)), a.n * int64_t(sizeof(O)), int(sizeof(O)),
+                     {FastDiv32(uint32_t(row_accesses(a.n, 16 / int(sizeof(O)), !on_grid)))}, a.vocab, 0, 0};
     if (a.ids->typenum == DPB_INT32) sort_ids<int32_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, zero, s);
     else sort_ids<int64_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, zero, s);
     take_zeros(zero, 0);
-    const int64_t zeroed = std::min(a.vocab * per_row, zero.first * access / int64_t(VEC * sizeof(O)));
+    // rows that are zero already (whole ones: the accesses of the sums may be others)
+    const int64_t zeroed = std::min(a.vocab, zero.first / zero.seq.per_row.d) * per_row;
     const int64_t sums = chunks * tiles, zeros = ceil_div(a.vocab * per_row - zeroed, kThreads * kAccesses);
     if (sums + zeros > 0) {
         const int64_t stride = sums > 0 ? std::max<int64_t>(1, (sums + zeros) / sums) : 1;
-        launch_after_previous(embedding_sums_kernel<T, O, VEC>, static_cast<unsigned>(sums + zeros), unsigned(kThreads), s,
-                              static_cast<const T *>(a.dout->data), a.dm, key, pos, uint32_t(a.tokens), mark, part, A(a.scale), dtable,
-                              a.ld, uint32_t(a.vocab), RowSequence{FastDiv32(uint32_t(per_row))}, uint32_t(sums),
-                              FastDiv32(uint32_t(tiles)), FastDiv32(uint32_t(stride)), zeroed, chunk);
+        launch_after_previous(embedding_sums_kernel<T, O, SHIFT>, static_cast<unsigned>(sums + zeros), unsigned(kThreads), s,
+                              static_cast<const T *>(a.dout->data), a.dm, a.tokens > 0 ? span_of<T>(*a.dout) : Span<T>{nullptr, nullptr},
+                              static_cast<const uint32_t *>(key), static_cast<const uint32_t *>(pos), uint32_t(a.tokens),
+                              static_cast<const uint8_t *>(mark), part, A(a.scale), dtable, a.ld, uint32_t(a.vocab), a.n,
+                              RowSequence{FastDiv32(uint32_t(per_row))}, uint32_t(sums), FastDiv32(uint32_t(tiles)),
+                              FastDiv32(uint32_t(stride)), zeroed, chunk);
         note_kernel("embedding_sums");
     }
     if (chunks < 2) return;
@@ -642,8 +721,8 @@ template <class T, class O, int VEC> static void run_sums(const EmbedGradArgs &a
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    cudaLaunchKernelEx(&cfg, embedding_join_kernel<A, O, VEC>, static_cast<const uint32_t *>(key), uint32_t(a.tokens),
-                       static_cast<const A *>(part), A(a.scale), dtable, a.ld, uint32_t(a.vocab), uint32_t(per_row), chunk);
+    cudaLaunchKernelEx(&cfg, embedding_join_kernel<A, O, VEC, SHIFT>, static_cast<const uint32_t *>(key), uint32_t(a.tokens),
+                       static_cast<const A *>(part), A(a.scale), dtable, a.ld, uint32_t(a.vocab), a.n, uint32_t(per_row), chunk);
     note_kernel("embedding_join");
 }
 
@@ -651,20 +730,21 @@ template <class T, class O> static int run_backward(const EmbedGradArgs &a, cuda
 {
     using A = acc_t<T>;
     constexpr int wide = vec_width<T>();
-    int v = a.tokens > 0 ? row_vector(a.dout->data, a.dm, a.n, sizeof(T), wide) : wide;
-    while (v > 1 && (a.n % v || a.ld % v || !is_aligned(a.dtable->data, v * sizeof(O)))) v /= 2;
+    const RowMap table = {0, a.ld, FastDiv32(1)};
+    const bool shift = (a.tokens > 0 && row_vector(a.dout->data, a.dm, a.n, sizeof(T), wide) != wide) ||
+                       row_vector(a.dtable->data, table, a.n, sizeof(O), wide) != wide;
+    const int64_t per_row = row_accesses(a.n, wide, shift);
     // long chunks leave fewer parts of frequent ids to add up, short ones give few tokens enough blocks
-    const int64_t tiles = ceil_div(ceil_div(a.n, v), kThreads);
+    const int64_t tiles = ceil_div(per_row, kThreads);
     uint32_t chunk = 32;
     while (chunk < kMaxChunk && a.tokens / (2 * chunk) * tiles >= 4 * device_props().sm_count) chunk *= 2;
     // sorted keys and positions, counters, a mark a row; parts of runs
     const size_t words = static_cast<size_t>(sort_words(a.tokens) + ceil_div(a.vocab, 4)) * 4;
     const size_t head = (words + 255) / 256 * 256;
     void *work = nullptr;
-    DPB_TRY(dpb_malloc(head + static_cast<size_t>(2 * ceil_div(a.tokens, int64_t(chunk)) * a.n) * sizeof(A), s, &work));
-    if (v == wide) run_sums<T, O, wide>(a, work, head, chunk, s);
-    else if (is_half_v<T> && v >= 2) run_sums<T, O, is_half_v<T> ? 2 : 1>(a, work, head, chunk, s);
-    else run_sums<T, O, 1>(a, work, head, chunk, s);
+    DPB_TRY(dpb_malloc(head + static_cast<size_t>(2 * ceil_div(a.tokens, int64_t(chunk)) * per_row * wide) * sizeof(A), s, &work));
+    if (shift) run_sums<T, O, true>(a, work, head, chunk, s);
+    else run_sums<T, O, false>(a, work, head, chunk, s);
     const int st = check_launch("embedding_backward");
     dpb_free(work, s);
     return st;

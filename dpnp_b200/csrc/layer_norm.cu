@@ -29,10 +29,6 @@ constexpr int kGroupThreads = 1024;   // threads an SM, at 64 registers
 
 enum Keep { kGlobal, kRegisters, kShared };
 
-template <class T> struct Span {
-    const T *lo, *hi;   // an array's elements
-};
-
 // Weight and bias of one thread's columns.
 template <class W, int VEC, int ITEMS> struct KeptWeights {
     static constexpr int parts = VEC * sizeof(W) > 16 ? VEC * static_cast<int>(sizeof(W)) / 16 : 1;

@@ -338,8 +338,6 @@ DPB_D float exp_(float a) { return expf(a); }
 DPB_D double exp_(double a) { return exp(a); }
 DPB_D float log_(float a) { return logf(a); }
 DPB_D double log_(double a) { return log(a); }
-DPB_D float sqrt_(float a) { return sqrtf(a); }
-DPB_D double sqrt_(double a) { return sqrt(a); }
 // 1 / sqrt(a): within 2 steps of float, 1 of double; a quotient and a root cost ten times the instructions
 DPB_D float rsqrt_(float a) { return rsqrtf(a); }
 DPB_D double rsqrt_(double a) { return rsqrt(a); }
@@ -514,6 +512,40 @@ template <class A, int N, class W> DPB_D void load_values(const W *p, Values<A, 
     }
 }
 
+// 16 bytes of elements from an address that is aligned to its elements only: the two aligned accesses around it,
+// shifted into place (about 15 instructions, against one load an element), where both lie in the array [lo, hi).
+template <class T, int VEC> DPB_D vec_t<T, VEC> load_anywhere(const T *p, const T *lo, const T *hi)
+{
+    using V = vec_t<T, VEC>;
+    static_assert(sizeof(V) == 16, "whole accesses");
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+    if (off == 0) return load_vec<V>(p);
+    const T *q = reinterpret_cast<const T *>(reinterpret_cast<uintptr_t>(p) - off);
+    V out;
+    if (q >= lo && q + 2 * VEC <= hi) {
+        const int4 a = __ldg(reinterpret_cast<const int4 *>(q)), b = __ldg(reinterpret_cast<const int4 *>(q) + 1);
+        uint32_t w[8] = {uint32_t(a.x), uint32_t(a.y), uint32_t(a.z), uint32_t(a.w),
+                         uint32_t(b.x), uint32_t(b.y), uint32_t(b.z), uint32_t(b.w)};
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+        if constexpr (sizeof(T) <= 4) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+        }
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+        }
+        int4 r = make_int4(int(w[0]), int(w[1]), int(w[2]), int(w[3]));
+        out = *reinterpret_cast<V *>(&r);
+    }
+    else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out.v[j] = p[j];
+    }
+    return out;
+}
+
 // ------------------------------------------------------------------- rows fetched ahead into shared memory
 // Copy of one access (16, 8 or 4 bytes) into shared memory that does not wait (2 bytes: a plain copy).
 template <class V> DPB_D void copy_async(V *shared, const V *global)
@@ -530,6 +562,10 @@ template <class V> DPB_D void copy_async(V *shared, const V *global)
 }
 DPB_D void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> DPB_D void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <class T> struct Span {
+    const T *lo, *hi;   // an array's elements
+};
 
 // The accesses of one thread to a row of n elements: ITEMS accesses of VEC elements, `width` threads apart.
 // Where a row starts `mis` elements behind a 16-byte boundary the accesses start at that boundary (the
