@@ -5,7 +5,9 @@ reduction-over-axis engine) on NVIDIA B200, behind the dpnp Python API.
 elementwise and reduction paths need: ``ndarray``, creation and view functions,
 the ufunc objects (add, subtract, multiply, divide, negative, exp, log, sqrt,
 erf, comparisons, ...), ``where``, and the reductions sum, prod, mean, max, min,
-argmax, argmin, plus ``fuse`` (a chain of elementwise calls as one launch).  All compute runs in hand-written CUDA kernels of
+argmax, argmin, ``fuse`` (a chain of elementwise calls as one launch), and operators over the
+rows of a matrix that surround a language model's matrix products: ``layer_norm``, ``embedding``,
+``distillation_loss`` and their gradients.  All compute runs in hand-written CUDA kernels of
 ``libdpnp_b200.so``; there is no CPU fallback.
 """
 
