@@ -37,6 +37,18 @@ struct RowSequence {
     }
 };
 
+// Rows shared out to groups of 2^bits threads of a block, as many as a row has accesses (rounded up to a power of two,
+// at most the block): no division at all, for the stores of zeros.
+constexpr int kRows = 4;   // of a thread
+
+struct RowGroups {
+    int bits;
+    DPB_HD int width() const { return 1 << bits; }
+    DPB_HD int groups() const { return kThreads >> bits; }
+    DPB_D uint32_t lane() const { return threadIdx.x & (width() - 1); }
+    DPB_D uint32_t group() const { return threadIdx.x >> bits; }
+};
+
 // Access k of a row that starts `mis` elements behind a 16-byte boundary begins at column k VEC - mis: all but the
 // first and the last are whole and aligned.  A row of n elements has at most n + VEC - 1 over VEC of them (rounded up).
 template <class T, int VEC> struct ShiftedColumn {
@@ -132,36 +144,42 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 512;
 constexpr int kJoinedTiles = 64;
 
-// Zeros for a range of a matrix's accesses: the sort occupies few SMs, and its launches carry blocks that
-// begin with the gradient's zeros (of rows that occur, too: they are written again later).
+// Zeros for some rows of a matrix: the sort occupies few SMs, and its launches carry blocks that begin with the
+// gradient's zeros (of rows that occur, too: they are written again later).
 struct ZeroRows {
     char *base;
     int64_t row_bytes;     // from one row to the next
     int64_t bytes;         // of a row
     int item;              // bytes of an element
-    RowSequence seq;       // accesses of 16 bytes, shifted to the rows' starts
-    int64_t rows, first;   // first access of this launch
+    RowGroups groups;      // accesses of 16 bytes, shifted to the rows' starts
+    int64_t rows, first;   // first row of this launch
     int64_t blocks;
+    DPB_HD int64_t block_rows() const { return int64_t(groups.groups()) * kRows; }
 };
-DPB_D void zero_rows(const ZeroRows &z, int64_t block)
+// `skip` (or null): rows that are written by others
+DPB_D void zero_rows(const ZeroRows &z, int64_t block, const uint8_t *skip)
 {
-    int64_t row;
-    uint32_t rest;
-    z.seq.start(z.first + block * (kThreads * kAccesses), row, rest);
+    const int64_t row0 = z.first + block * z.block_rows() + z.groups.group();
+    bool mine[kRows];
 #pragma unroll
-    for (int k = 0; k < kAccesses; ++k) {
-        uint32_t q, c;
-        z.seq.per_row.divmod(rest + k * kThreads + threadIdx.x, q, c);
-        if (row + q >= z.rows) continue;
-        char *start = z.base + (row + q) * z.row_bytes;
-        const int64_t at = int64_t(c) * 16 - int64_t(reinterpret_cast<uintptr_t>(start) % 16);
-        if (at >= 0 && at + 16 <= z.bytes) *reinterpret_cast<int4 *>(start + at) = make_int4(0, 0, 0, 0);
-        else
-            for (int64_t i = max(at, int64_t(0)); i < min(at + 16, z.bytes); i += z.item) {
-                if (z.item == 2) *reinterpret_cast<short *>(start + i) = 0;
-                else if (z.item == 4) *reinterpret_cast<int *>(start + i) = 0;
-                else *reinterpret_cast<long long *>(start + i) = 0;
-            }
+    for (int k = 0; k < kRows; ++k) {
+        const int64_t row = row0 + k * z.groups.groups();
+        mine[k] = row < z.rows && !(skip && skip[row]);
+    }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+        if (!mine[k]) continue;
+        char *start = z.base + (row0 + k * z.groups.groups()) * z.row_bytes;
+        const int64_t mis = static_cast<int64_t>(reinterpret_cast<uintptr_t>(start) % 16);
+        for (int64_t at = int64_t(z.groups.lane()) * 16 - mis; at < z.bytes; at += int64_t(z.groups.width()) * 16) {
+            if (at >= 0 && at + 16 <= z.bytes) *reinterpret_cast<int4 *>(start + at) = make_int4(0, 0, 0, 0);
+            else
+                for (int64_t i = max(at, int64_t(0)); i < min(at + 16, z.bytes); i += z.item) {
+                    if (z.item == 2) *reinterpret_cast<short *>(start + i) = 0;
+                    else if (z.item == 4) *reinterpret_cast<int *>(start + i) = 0;
+                    else *reinterpret_cast<long long *>(start + i) = 0;
+                }
+        }
     }
 }
 
@@ -245,7 +263,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortIn in, boo
 {
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
     cudaGridDependencySynchronize();
-    if (blockIdx.x >= tiles) return zero_rows(zero, blockIdx.x - tiles);
+    if (blockIdx.x >= tiles) return zero_rows(zero, blockIdx.x - tiles, nullptr);
     SortItems it;
     load_items<I>(in, first, n, vocab, it);
     const int digits = 1 << bits;
@@ -336,7 +354,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortIn in, boo
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
     __shared__ uint32_t place[kMaxDigits], warp_sum[kSortWarps];
     cudaGridDependencySynchronize();
-    if (blockIdx.x >= tiles) return zero_rows(zero, blockIdx.x - tiles);
+    if (blockIdx.x >= tiles) return zero_rows(zero, blockIdx.x - tiles, nullptr);
     SortItems it;
     load_items<I>(in, first, n, vocab, it);
     const int digits = 1 << bits, d0 = 2 * threadIdx.x;
@@ -388,7 +406,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const I *ids, i
     __shared__ uint32_t count[kSortWarps][kMaxDigits];
     __shared__ uint32_t place[kMaxDigits], warp_sum[kSortWarps], keys[kTile], positions[kTile];
     cudaGridDependencySynchronize();
-    if (blockIdx.x >= 1) return zero_rows(zero, blockIdx.x - 1);
+    if (blockIdx.x >= 1) return zero_rows(zero, blockIdx.x - 1, nullptr);
     SortItems it;
     load_items<I>({ids, nullptr, nullptr}, true, n, vocab, it);
     for (int64_t i = threadIdx.x; i < marks; i += kSortThreads) reinterpret_cast<uint32_t *>(mark)[i] = 0;
@@ -435,15 +453,14 @@ constexpr int kInFlight = 8;    // rows' loads of a thread in flight
 
 // The first blocks sum runs: block (chunk k, column tile) walks its tokens in order.  A run that lies in the chunk goes
 // to the table; part[2 k] takes the sum of one that came in from chunk k - 1 (and may go on), part[2 k + 1]
-// of one that starts here and goes on.  The other blocks write the rows that do not occur (from access `zeroed`
-// on), kAccesses accesses a thread.  Every `stride`-th block is one of the first kind: reads and writes
-// overlap.
+// of one that starts here and goes on.  The other blocks write the rows that do not occur.  Every `stride`-th block
+// is one of the first kind: reads and writes overlap.
 template <class T, class O, bool SHIFT>
 __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout, RowMap dm, Span<T> array, const uint32_t *key,
                                                                   const uint32_t *pos, uint32_t tokens, const uint8_t *mark,
                                                                   acc_t<T> *part, acc_t<T> scale, O *dtable, int64_t ld,
-                                                                  uint32_t vocab, int64_t n, RowSequence seq, uint32_t sum_blocks,
-                                                                  FastDiv32 tiles, FastDiv32 stride, int64_t zeroed, uint32_t chunk)
+                                                                  uint32_t vocab, int64_t n, uint32_t per_row, uint32_t sum_blocks,
+                                                                  FastDiv32 tiles, FastDiv32 stride, ZeroRows zero, uint32_t chunk)
 {
     using A = acc_t<T>;
     constexpr int VEC = vec_width<T>(), flight = SHIFT ? kInFlight / 2 : kInFlight;
@@ -459,21 +476,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
     cudaGridDependencySynchronize();
     uint32_t block, off;
     stride.divmod(blockIdx.x, block, off);
-    if (off != 0 || block >= sum_blocks) {
-        int64_t row;
-        uint32_t rest;
-        seq.start(zeroed + int64_t(blockIdx.x - min(block + (off != 0), sum_blocks)) * (kThreads * kAccesses), row, rest);
-        Vals zero;
-        zero.fill(0);
-#pragma unroll
-        for (int k = 0; k < kAccesses; ++k) {
-            uint32_t q, c;
-            seq.per_row.divmod(rest + k * kThreads + threadIdx.x, q, c);
-            const int64_t v = row + q;
-            if (v < vocab && !mark[v]) write(v, c, zero);
-        }
-        return;
-    }
+    if (off != 0 || block >= sum_blocks) return zero_rows(zero, blockIdx.x - min(block + (off != 0), sum_blocks), mark);
     __shared__ uint32_t keys[kMaxChunk + 2];   // with the token before and the token behind the chunk
     __shared__ int64_t rows[kMaxChunk];
     uint32_t k, tile;
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
     if (threadIdx.x < count) rows[threadIdx.x] = dm(pos[begin + threadIdx.x]);
     __syncthreads();
     const uint32_t c = tile * kThreads + threadIdx.x;
-    if (c >= seq.per_row.d) return;
+    if (c >= per_row) return;
     Vals s, u;
     s.fill(0);
     bool whole = keys[0] != keys[1];   // the current run starts in this chunk
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
                 s.mul(scale);
                 write(id, c, s);
             }
-            else *reinterpret_cast<Vals *>(part + (int64_t(2 * k + whole) * seq.per_row.d + c) * VEC) = s;
+            else *reinterpret_cast<Vals *>(part + (int64_t(2 * k + whole) * per_row + c) * VEC) = s;
             s.fill(0);
             whole = true;
         }
@@ -562,11 +565,6 @@ struct EmbedArgs {
     double scale;
 };
 
-static unsigned sequence_blocks(int64_t rows, int64_t per_row)
-{
-    return static_cast<unsigned>(ceil_div(rows * per_row, kThreads * kAccesses));
-}
-
 // Accesses of 16 bytes a row: without and with a shift to the row's start (two partial ones then).
 static int64_t row_accesses(int64_t n, int vec, bool shift)
 {
@@ -578,6 +576,18 @@ template <class T> static Span<T> span_of(const dpb_array &a)
     const void *lo, *hi;
     array_bounds(a, lo, hi);
     return {static_cast<const T *>(lo), static_cast<const T *>(hi)};
+}
+
+static RowGroups row_groups(int64_t per_row)
+{
+    RowGroups g = {0};
+    while (g.width() < kThreads && g.width() < per_row) ++g.bits;
+    return g;
+}
+
+static unsigned sequence_blocks(int64_t rows, int64_t per_row)
+{
+    return static_cast<unsigned>(ceil_div(rows * per_row, kThreads * kAccesses));
 }
 
 template <class T, class I, bool SHIFT> static void launch_forward(const EmbedArgs &a, cudaStream_t s)
@@ -613,9 +623,9 @@ constexpr int64_t kZerosCounting = int64_t(32) << 20, kZerosPlacing = int64_t(64
 // Moves `zero` on to the next launch's share, of `bytes` at most; its number of blocks.
 static int64_t take_zeros(ZeroRows &z, int64_t bytes)
 {
-    z.first += z.blocks * (kThreads * kAccesses);
-    const int64_t left = std::max<int64_t>(0, z.rows * z.seq.per_row.d - z.first);
-    z.blocks = ceil_div(std::min(left, bytes / 16), kThreads * kAccesses);
+    z.first = std::min(z.rows, z.first + z.blocks * z.block_rows());
+    const int64_t rows = std::min(z.rows - z.first, bytes / z.bytes);
+    z.blocks = rows == z.rows - z.first ? ceil_div(rows, z.block_rows()) : rows / z.block_rows();
     return z.blocks;
 }
 
@@ -690,23 +700,18 @@ static void run_sums(const EmbedGradArgs &a, void *work, size_t head, uint32_t c
     A *part = reinterpret_cast<A *>(static_cast<char *>(work) + head);
     const int64_t per_row = row_accesses(a.n, VEC, SHIFT), tiles = ceil_div(per_row, kThreads), chunks = ceil_div(a.tokens, int64_t(chunk));
     O *dtable = static_cast<O *>(a.dtable->data);
-    const bool on_grid = !SHIFT && a.n * sizeof(O) % 16 == 0;
     ZeroRows zero = {reinterpret_cast<char *>(dtable), a.ld * int64_t(sizeof(O)), a.n * int64_t(sizeof(O)), int(sizeof(O)),
-                     {FastDiv32(uint32_t(row_accesses(a.n, 16 / int(sizeof(O)), !on_grid)))}, a.vocab, 0, 0};
+                     row_groups(row_accesses(a.n, 16 / int(sizeof(O)), SHIFT || a.n * sizeof(O) % 16 != 0)), a.vocab, 0, 0};
     if (a.ids->typenum == DPB_INT32) sort_ids<int32_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, zero, s);
     else sort_ids<int64_t>(a.ids->data, a.tokens, a.vocab, w, mark, key, pos, zero, s);
-    take_zeros(zero, 0);
-    // rows that are zero already (whole ones: the accesses of the sums may be others)
-    const int64_t zeroed = std::min(a.vocab, zero.first / zero.seq.per_row.d) * per_row;
-    const int64_t sums = chunks * tiles, zeros = ceil_div(a.vocab * per_row - zeroed, kThreads * kAccesses);
+    const int64_t sums = chunks * tiles, zeros = take_zeros(zero, INT64_MAX);
     if (sums + zeros > 0) {
         const int64_t stride = sums > 0 ? std::max<int64_t>(1, (sums + zeros) / sums) : 1;
         launch_after_previous(embedding_sums_kernel<T, O, SHIFT>, static_cast<unsigned>(sums + zeros), unsigned(kThreads), s,
                               static_cast<const T *>(a.dout->data), a.dm, a.tokens > 0 ? span_of<T>(*a.dout) : Span<T>{nullptr, nullptr},
                               static_cast<const uint32_t *>(key), static_cast<const uint32_t *>(pos), uint32_t(a.tokens),
                               static_cast<const uint8_t *>(mark), part, A(a.scale), dtable, a.ld, uint32_t(a.vocab), a.n,
-                              RowSequence{FastDiv32(uint32_t(per_row))}, uint32_t(sums), FastDiv32(uint32_t(tiles)),
-                              FastDiv32(uint32_t(stride)), zeroed, chunk);
+                              uint32_t(per_row), uint32_t(sums), FastDiv32(uint32_t(tiles)), FastDiv32(uint32_t(stride)), zero, chunk);
         note_kernel("embedding_sums");
     }
     if (chunks < 2) return;
