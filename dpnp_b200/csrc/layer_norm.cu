@@ -5,8 +5,9 @@
 //
 // Means, variances and all sums are float (double for float64 data); every result is rounded once.
 // The variance is the mean of squared deviations from the mean (two sweeps over the row), not
-// E[x^2] - m^2, which loses all digits of rows far from zero.  Every term is divided by n as it is added
-// (one multiplication, fused where it can be), so that a sum overflows only where the mean itself does.
+// E[x^2] - m^2, which loses all digits of rows far from zero.  A sum overflows only where the mean itself
+// does: every term of float32 and float64 data is divided by n as it is added (one multiplication, fused
+// where it can be); float16 data cannot overflow a float32 sum.
 #include "row_ops.cuh"
 
 namespace dpb {
@@ -19,12 +20,10 @@ constexpr int kThreads = 256;
 // and the instructions around them, not the bytes: R rows share the folds, and the arithmetic is done in
 // pairs.  Rows are copied into shared memory ahead of their use (each thread its own accesses: no barrier),
 // DEPTH - 1 rounds or, with one slot, from the moment that the rows before are in registers; that keeps 32 to
-// 64 KiB an SM in flight.  The rows that are summed stay in registers as numbers of the accumulation type.  Weight and bias are kept for all rows of a group, in
-// registers or (KEEP = kShared) in the thread's own slots of shared memory: from L1 they cost more
-// transfers than the data when they are float32 and the data float16.
-//
-// float16 data cannot overflow a float32 sum, so the division by n waits until after the sum there; other
-// data is divided term by term.
+// 64 KiB an SM in flight.  The rows that are summed stay in registers as numbers of the accumulation type.
+// Weight and bias are kept for all rows of a group, in registers or (KEEP = kShared) in the thread's own
+// slots of shared memory: from L1 they cost more transfers than the data when they are float32 and the data
+// float16.
 constexpr int kGroupThreads = 1024;   // threads an SM, at 64 registers
 
 enum Keep { kGlobal, kRegisters, kShared };
