@@ -527,15 +527,17 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const T *dout,
 template <class A, class O, int VEC, bool SHIFT>
 __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t *key, uint32_t tokens, const A *part, A scale,
                                                                   O *dtable, int64_t ld, uint32_t vocab, int64_t n,
-                                                                  uint32_t per_row, uint32_t chunk)
+                                                                  uint32_t per_row, FastDiv32 tiles, uint32_t chunk)
 {
     using Vals = Values<A, VEC>;
     cudaGridDependencySynchronize();
-    const uint32_t k = blockIdx.x + 1, begin = k * chunk, end = min(tokens, begin + chunk);
+    uint32_t before, tile;
+    tiles.divmod(blockIdx.x, before, tile);
+    const uint32_t k = before + 1, begin = k * chunk, end = min(tokens, begin + chunk);
     const uint32_t id = key[begin];
     // a run that came in and ends here
     if (id >= vocab || key[begin - 1] != id || (end < tokens && key[end - 1] == id && key[end] == id)) return;
-    const uint32_t c = blockIdx.y * kThreads + threadIdx.x;
+    const uint32_t c = tile * kThreads + threadIdx.x;
     // chunks before this one whose last token belongs to the run, a warp at a time
     uint32_t first = k;   // the first chunk that the run came into
     for (;;) {
@@ -715,19 +717,9 @@ static void run_sums(const EmbedGradArgs &a, void *work, size_t head, uint32_t c
         note_kernel("embedding_sums");
     }
     if (chunks < 2) return;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(chunks - 1), static_cast<unsigned>(tiles));
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    if (tuning_pdl()) {
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-    }
-    cudaLaunchKernelEx(&cfg, embedding_join_kernel<A, O, VEC, SHIFT>, static_cast<const uint32_t *>(key), uint32_t(a.tokens),
-                       static_cast<const A *>(part), A(a.scale), dtable, a.ld, uint32_t(a.vocab), a.n, uint32_t(per_row), chunk);
+    launch_after_previous(embedding_join_kernel<A, O, VEC, SHIFT>, static_cast<unsigned>((chunks - 1) * tiles), unsigned(kThreads), s,
+                          static_cast<const uint32_t *>(key), uint32_t(a.tokens), static_cast<const A *>(part), A(a.scale), dtable, a.ld,
+                          uint32_t(a.vocab), a.n, uint32_t(per_row), FastDiv32(uint32_t(tiles)), chunk);
     note_kernel("embedding_join");
 }
 

@@ -472,6 +472,18 @@ def test_embedding_backward_long_batches(tokens, rows, n, idt):
     assert np.array_equal(host(again), host(got))
 
 
+@pytest.mark.parametrize("n", [5000, 20011])
+@pytest.mark.parametrize("dt", ["f2", "f4"])
+def test_embedding_backward_frequent_ids_of_wide_rows(dt, n):
+    """Runs over several chunks, in rows of several blocks."""
+    import dpnp_b200 as dp
+
+    rng = np.random.default_rng(n)
+    ids = np.where(rng.uniform(0, 1, 400) < 0.6, 3, rng.integers(-1, 6, 400)).astype("i4")
+    dout = rng.normal(0, 1, (400, n)).astype(dt)
+    check_embedding_backward(dout, ids, 7, 0.5, host(dp.embedding_backward(dev(dout), dev(ids), 7, scale=0.5)), dt)
+
+
 def test_embedding_backward_layouts():
     import dpnp_b200 as dp
 
