@@ -40,12 +40,12 @@ constexpr double kLog2E = 1.4426950408889634074;
 
 // Exponentials of a row's values below its largest one, T given as k = log2(e) / T.
 //
-// float and double: 2^((v - top) k), the difference taken first, so that values of the type's lowest number do not
-// overflow.  float16: 2^(v k - c) with c = top k rounded, which is one fused operation a value; what c is off by
-// (rest) is exact and corrects the sum once.  `finite`: what a row whose values are all -inf is reduced by.
-template <class T> struct Exponent {
+// 2^((v - top) k), the difference taken first, so that values of the type's lowest number do not overflow.  FUSED,
+// for float16: 2^(v k - c) with c = top k rounded, which is one operation a value; what c is off by (rest) is exact
+// and corrects the sum once.  `finite`: what a row whose values are all -inf is reduced by.
+template <class T, bool FUSED> struct Exponent {
     using A = acc_t<T>;
-    static constexpr bool fused = is_half_v<T>;
+    static constexpr bool fused = FUSED;
     A k, base;
     static DPB_D A finite(A t) { return t == -INFINITY ? A(0) : t; }
     DPB_D Exponent(A top, A k_) : k(k_), base(fused ? -(finite(top) * k_) : -finite(top)) {}
@@ -73,16 +73,17 @@ template <class T> struct Exponent {
 };
 
 // The largest of some values and the sum of their exponentials.
-template <class T> struct alignas(2 * sizeof(acc_t<T>)) SoftSum {
+template <class T, bool FUSED> struct alignas(2 * sizeof(acc_t<T>)) SoftSum {
     using A = acc_t<T>;
+    using Exp = Exponent<T, FUSED>;
     A top, sum;
     DPB_D void raise(A to, A k)   // to >= top
     {
-        if constexpr (Exponent<T>::fused) {
-            const A factor = exp2_<true>(Exponent<T>(to, k).base - Exponent<T>(top, k).base);
+        if constexpr (FUSED) {
+            const A factor = exp2_<true>(Exp(to, k).base - Exp(top, k).base);
             sum = top == -INFINITY ? A(0) : sum * factor;
         }
-        else sum *= exp2_<true>((top - Exponent<T>::finite(to)) * k);
+        else sum *= exp2_<true>((top - Exp::finite(to)) * k);
         top = to;
     }
     DPB_D SoftSum over_warp(A k) const
@@ -94,7 +95,7 @@ template <class T> struct alignas(2 * sizeof(acc_t<T>)) SoftSum {
     }
     DPB_D A log_sum(A k) const   // log sum exp((v - top) / T)
     {
-        return log_(sum) - Exponent<T>(top, k).rest(top) * A(0.69314718055994530942);
+        return log_(sum) - Exp(top, k).rest(top) * A(0.69314718055994530942);
     }
 };
 
@@ -203,12 +204,12 @@ template <class T> struct RowSplit {
 
 // The gradient of a row's columns, dloss T (q - weight): q is an exponential times `scale` (0 in a row whose logits
 // are all -inf).
-template <class T> struct RowGradient {
+template <class T, bool FUSED> struct RowGradient {
     using A = acc_t<T>;
     static constexpr bool ftz = is_half_v<T>;   // (float16 has no numbers as small as those that are flushed)
-    Exponent<T> ex;
+    Exponent<T, FUSED> ex;
     A scale, g;
-    DPB_D RowGradient(const SoftSum<T> &s, A k, A g_) : ex(s.top, k), scale(s.sum == 0 ? A(0) : g_ / s.sum), g(g_) {}
+    DPB_D RowGradient(const SoftSum<T, FUSED> &s, A k, A g_) : ex(s.top, k), scale(s.sum == 0 ? A(0) : g_ / s.sum), g(g_) {}
     DPB_D RowGradient(A top, A log_sum, A k, A g_)   // from kept statistics
         : ex(top, k), scale(log_sum == -INFINITY ? A(0) : g_ * exp_(-log_sum) * exp2_<false>(-ex.rest(top))), g(g_)
     {
@@ -286,7 +287,7 @@ template <class T, class I> struct RowPart {
         for (int i = threadIdx.x; i < split.mine; i += blockDim.x) put(out, i, z, whole);
         if (single >= 0) out[single] = z.v[0];
     }
-    DPB_D void dense_gradient(T *out, const RowGradient<T> &grad) const
+    template <bool FUSED> DPB_D void dense_gradient(T *out, const RowGradient<T, FUSED> &grad) const
     {
         const bool whole = aligned(out);
         const int threads = blockDim.x;
@@ -308,7 +309,7 @@ template <class T, class I> struct RowPart {
         if (single >= 0) out[single] = from_acc<T>(grad.at(to_acc<A>(row[single]), A(0)));
     }
     // The teacher's columns of this part once more, with its weight taken off (after a barrier).
-    DPB_D void teacher_gradient(T *out, const RowGradient<T> &grad) const
+    template <bool FUSED> DPB_D void teacher_gradient(T *out, const RowGradient<T, FUSED> &grad) const
     {
         for (int i = threadIdx.x; i < k; i += blockDim.x) {
             const int c = teacher.at[i];
@@ -329,7 +330,7 @@ template <class T, class I> struct RowPart {
 //
 // Two exponentials an element: at float16 and the copy rate that is 3.3e12 a second, three quarters of what the
 // special function units give; the rest of the arithmetic is done in pairs to stay out of their way.
-template <class T, class I, bool GRAD>
+template <class T, class I, bool GRAD, bool FUSED>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
     distillation_row_kernel(const T *z, RowMap zm, const acc_t<T> *top, const I *index, int k, int vocab, acc_t<T> temp,
                             acc_t<T> inv_temp, acc_t<T> exp_scale, acc_t<T> *loss, acc_t<T> *stats, const acc_t<T> *dloss,
@@ -337,10 +338,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
 {
     using A = acc_t<T>;
     using Part = RowPart<T, I>;
+    using Sum = SoftSum<T, FUSED>;
     using V = typename Part::V;
     constexpr int VEC = Part::VEC;
     extern __shared__ __align__(16) char shared_bytes[];
-    __shared__ SoftSum<T> warp_sums[kThreads / 32], rank_sums[kMaxRanks];
+    __shared__ Sum warp_sums[kThreads / 32], rank_sums[kMaxRanks];
     __shared__ A buf[kThreads / 32];
     __shared__ int used;
     cudaGridDependencySynchronize();
@@ -356,8 +358,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
         if constexpr (GRAD) part.zeros(out);
         return;
     }
+    // (waited for before the first write into another block's memory: that block has to have begun)
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const A alone = part.single >= 0 ? to_acc<A>(part.row[part.single]) : A(-INFINITY);
-    SoftSum<T> s = {alone, part.single >= 0 ? Exponent<T>(alone, exp_scale).template exp<true>(alone) : A(0)};
+    Sum s = {alone, part.single >= 0 ? Exponent<T, FUSED>(alone, exp_scale).template exp<true>(alone) : A(0)};
     const V *from = part.from();
     V low;
 #pragma unroll
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
 #pragma unroll
         for (int f = 1; f < kInFlight; ++f) best = max_nan(best, largest<T, VEC>(raw[f]));
         s.raise(max_nan(s.top, best), exp_scale);
-        const Exponent<T> ex(s.top, exp_scale);
+        const Exponent<T, FUSED> ex(s.top, exp_scale);
         auto sum = Values<A, VEC>::all(0);
 #pragma unroll
         for (int f = 0; f < kInFlight; ++f) {
@@ -387,9 +391,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
     s = s.over_warp(exp_scale);
     if (lane == 0) warp_sums[warp] = s;
     __syncthreads();
-    s = lane < threads / 32 ? warp_sums[lane] : SoftSum<T>{-INFINITY, 0};
+    s = lane < threads / 32 ? warp_sums[lane] : Sum{-INFINITY, 0};
     s = s.over_warp(exp_scale);
     if (ranks > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         // every rank writes its sum to every rank; the barrier of the cluster makes them visible (and follows the reads
         // of read_at_teacher)
         if (threadIdx.x < ranks) {
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        s = lane < ranks ? rank_sums[lane] : SoftSum<T>{-INFINITY, 0};
+        s = lane < ranks ? rank_sums[lane] : Sum{-INFINITY, 0};
         s = s.over_warp(exp_scale);
     }
     if (rank == 0) {
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
         }
     }
     if constexpr (GRAD) {
-        const RowGradient<T> grad(s, exp_scale, dloss[r * dstep] * temp);
+        const RowGradient<T, FUSED> grad(s, exp_scale, dloss[r * dstep] * temp);
         part.dense_gradient(out, grad);
         __syncthreads();
         part.teacher_gradient(out, grad);
@@ -434,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
 
 // ------------------------------------------------------------------------------------------ gradient alone
 // From kept statistics: the same parts, without exchange.
-template <class T, class I>
+template <class T, class I, bool FUSED>
 __global__ void __launch_bounds__(kThreads)
     distillation_grad_kernel(const acc_t<T> *dloss, int64_t dstep, const T *z, RowMap zm, const acc_t<T> *top, const I *index, int k,
                              int vocab, acc_t<T> temp, acc_t<T> inv_temp, acc_t<T> exp_scale, const acc_t<T> *stats, T *dz,
@@ -450,7 +455,7 @@ __global__ void __launch_bounds__(kThreads)
     if (!part.read_teacher(top + int64_t(r) * k, index + int64_t(r) * k, used)) return part.zeros(out);
     part.read_at_teacher(false);
     __syncthreads();
-    const RowGradient<T> grad(stats[2 * int64_t(r)], stats[2 * int64_t(r) + 1], exp_scale, dloss[r * dstep] * temp);
+    const RowGradient<T, FUSED> grad(stats[2 * int64_t(r)], stats[2 * int64_t(r) + 1], exp_scale, dloss[r * dstep] * temp);
     part.dense_gradient(out, grad);
     if (threadIdx.x < 32) part.teacher.normalize(k, inv_temp);
     __syncthreads();
@@ -487,14 +492,14 @@ static unsigned share_threads(const Shares &share)
     return threads;
 }
 
-template <class T, class I> static int run_grad(const DistilArgs &a, cudaStream_t s)
+template <class T, class I, bool FUSED> static int run_grad(const DistilArgs &a, cudaStream_t s)
 {
     using A = acc_t<T>;
     Shares share;
     // parts of 64 to 128 KiB: below that the teacher's entries, which every block reads, show (1024 x 150001 float32:
     // 221 us at 75 KiB, 266 us at 37 KiB)
     DPB_TRY(share_row(a, sizeof(T), 128 * 1024, 10, share));
-    launch_shared(distillation_grad_kernel<T, I>, static_cast<unsigned>(a.rows << share.bits), share_threads(share),
+    launch_shared(distillation_grad_kernel<T, I, FUSED>, static_cast<unsigned>(a.rows << share.bits), share_threads(share),
                   RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const A *>(a.dloss->data), a.dloss->nd == 0 ? 0 : 1,
                   static_cast<const T *>(a.z->data), a.zm, static_cast<const A *>(a.top->data),
                   static_cast<const I *>(a.index->data), static_cast<int>(a.k), static_cast<int>(a.vocab), A(a.temp),
@@ -503,7 +508,7 @@ template <class T, class I> static int run_grad(const DistilArgs &a, cudaStream_
     return check_launch("distillation_grad");
 }
 
-template <class T, class I, bool GRAD> static int run_rows(const DistilArgs &a, cudaStream_t s)
+template <class T, class I, bool GRAD, bool FUSED> static int run_rows(const DistilArgs &a, cudaStream_t s)
 {
     using A = acc_t<T>;
     Shares share;
@@ -511,7 +516,7 @@ template <class T, class I, bool GRAD> static int run_rows(const DistilArgs &a, 
     // gradient 421 with quarters, 477 with halves (what the clusters hold has to stay in the cache between the
     // two readings)
     DPB_TRY(share_row(a, sizeof(T), (GRAD ? 64 : 256) * 1024, 3, share));
-    launch_cluster(distillation_row_kernel<T, I, GRAD>, static_cast<unsigned>(a.rows << share.bits), 1u << share.bits, share_threads(share),
+    launch_cluster(distillation_row_kernel<T, I, GRAD, FUSED>, static_cast<unsigned>(a.rows << share.bits), 1u << share.bits, share_threads(share),
                    RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const T *>(a.z->data), a.zm,
                    static_cast<const A *>(a.top->data), static_cast<const I *>(a.index->data), static_cast<int>(a.k),
                    static_cast<int>(a.vocab), A(a.temp), A(1.0 / a.temp), A(kLog2E / a.temp),
@@ -522,10 +527,20 @@ template <class T, class I, bool GRAD> static int run_rows(const DistilArgs &a, 
     return check_launch("distillation_row");
 }
 
+template <class T, class I, bool FUSED> static int run_as(const DistilArgs &a, cudaStream_t s)
+{
+    if (a.dz && !a.loss) return run_grad<T, I, FUSED>(a, s);
+    return a.dz ? run_rows<T, I, true, FUSED>(a, s) : run_rows<T, I, false, FUSED>(a, s);
+}
+
 template <class T, class I> static int run(const DistilArgs &a, cudaStream_t s)
 {
-    if (a.dz && !a.loss) return run_grad<T, I>(a, s);
-    return a.dz ? run_rows<T, I, true>(a, s) : run_rows<T, I, false>(a, s);
+    if constexpr (is_half_v<T>) {
+        // While the largest float16 divided by T (in powers of two) is below 2^24, its rounding is at most half a power
+        // of two.  Colder, the factor that corrects it would leave the range of float.
+        if (65504 * kLog2E / a.temp < 16777216) return run_as<T, I, true>(a, s);
+    }
+    return run_as<T, I, false>(a, s);
 }
 
 static int run_typed(const DistilArgs &a, cudaStream_t s)

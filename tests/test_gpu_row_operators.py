@@ -624,6 +624,15 @@ def test_distillation_many_rows_and_long_rows(dt):
         run_distil(z, t, idx, 1.5, rng.uniform(0.5, 2, rows).astype(ACC[dt]))
 
 
+@pytest.mark.parametrize("temp", [1e-10, 1e-6, 1e-4, 5.6e-3, 6e-3, 100.0, 1e6])
+@pytest.mark.parametrize("dt", TYPES)
+def test_distillation_temperatures(dt, temp):
+    """Far from 1, with small logits and with ones near the end of float16."""
+    for rows, vocab, scale in ((7, 1003, 1.0), (5, 1000, 6000.0), (2, 40000, 4000.0)):
+        z, t, idx, rng = distil_data(rows, vocab, 9, dt, vocab)
+        run_distil((z * scale).astype(dt), t, idx, temp, rng.uniform(0.5, 2, rows).astype(ACC[dt]))
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("idt", IDS)
 def test_distillation_types_and_shapes(dt, idt):
