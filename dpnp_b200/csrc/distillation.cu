@@ -4,7 +4,7 @@
 // and t > -inf.  With a temperature T,
 //   p = softmax(t / T) over the entries that count,  q = softmax(z / T),
 //   loss = T^2 sum_k p_k (log p_k - log q_{j_k}),    dz = dloss T (q - sum_{k: j_k = .} p_k).
-// A row without entries (padding, a prompt) has loss 0 and gradient 0, and its logits are not read.
+// A row without entries (padding, a prompt) has loss 0 and gradient 0, whatever its logits.
 // Where q is 0 (z = -inf, or every z of the row) and p is not, the loss is +inf; q counts as 0 in dz.
 //
 // log q = (z - max z) / T - log sum exp((z - max z) / T): the differences are taken before the
@@ -123,11 +123,11 @@ template <class A> struct Teacher {
     int *at;
     static DPB_HD size_t bytes(int k) { return size_t(k) * (2 * sizeof(A) + sizeof(int)) + 16; }
     DPB_D Teacher(void *shared, int k) : p(static_cast<A *>(shared)), logp(p + k), at(reinterpret_cast<int *>(logp + k)) {}
-    // One warp reads the entries; false when none counts.
+    // The block reads the entries (thread t every blockDim.x-th from t on); false for all when none counts.
     template <class I> DPB_D bool read(const A *top, const I *index, int k, int vocab) const
     {
         bool any = false;
-        for (int i = threadIdx.x & 31; i < k; i += 32) {
+        for (int i = threadIdx.x; i < k; i += blockDim.x) {
             const A v = top[i];
             const int64_t j = static_cast<int64_t>(index[i]);
             const bool counts = j >= 0 && j < vocab && !(v == -INFINITY);
@@ -135,9 +135,9 @@ template <class A> struct Teacher {
             logp[i] = v;
             any = any || counts;
         }
-        return __any_sync(0xffffffffu, any);
+        return __syncthreads_or(any);
     }
-    // The same warp turns them into probabilities.
+    // One warp turns them into probabilities.
     DPB_D void normalize(int k, A inv_temp) const
     {
         const int lane = threadIdx.x & 31;
@@ -248,24 +248,11 @@ template <class T, class I> struct RowPart {
     {
         return (c >= split.first && c < split.first + split.mine * VEC) || (c >= 0 && c < split.head) || c >= vocab - split.tail;
     }
-    // The first warp reads the teacher's entries.  Whether one counts, for the whole block.
-    DPB_D bool read_teacher(const A *top, const I *index, int &used) const
+    // The student's logit at the column of an entry that this thread has read (`all`, or this part's).
+    DPB_D T student(int i, bool all) const
     {
-        if (threadIdx.x < 32) {
-            const bool any = teacher.read(top, index, k, vocab);
-            if (threadIdx.x == 0) used = any;
-        }
-        __syncthreads();
-        return used;
-    }
-    // The first warp reads the logits at the teacher's columns (`all`, or this part's), before any block writes over them.
-    DPB_D void read_at_teacher(bool all) const
-    {
-        if (threadIdx.x >= 32) return;
-        for (int i = threadIdx.x; i < k; i += 32) {
-            const int c = teacher.at[i];
-            if (c >= 0 && (all || owns(c))) at_teacher[i] = to_acc<A>(row[c]);
-        }
+        const int c = i < k ? teacher.at[i] : -1;
+        return c >= 0 && (all || owns(c)) ? row[c] : from_acc<T>(A(0));
     }
     DPB_D const V *from() const { return reinterpret_cast<const V *>(row + split.first); }
     // Stores that are not read again here: they leave the cache first.
@@ -287,7 +274,11 @@ template <class T, class I> struct RowPart {
         for (int i = threadIdx.x; i < split.mine; i += blockDim.x) put(out, i, z, whole);
         if (single >= 0) out[single] = z.v[0];
     }
-    template <bool FUSED> DPB_D void dense_gradient(T *out, const RowGradient<T, FUSED> &grad) const
+    // Whether the part starts on a cache line.
+    DPB_D bool on_lines() const { return reinterpret_cast<uintptr_t>(from()) % 128 == 0; }
+    // LAST: lines leave the cache as they are read (16384 x 32000 float16: 358 us against 370), but not where two warps
+    // share a line, which the second would miss (16384 x 50257 float16: 671 us against 636).
+    template <bool LAST, bool FUSED> DPB_D void dense_gradient(T *out, const RowGradient<T, FUSED> &grad) const
     {
         const bool whole = aligned(out);
         const int threads = blockDim.x;
@@ -296,7 +287,10 @@ template <class T, class I> struct RowPart {
             V raw[kInFlight];
 #pragma unroll
             for (int f = 0; f < kInFlight; ++f)
-                if (i0 + f * threads < split.mine) raw[f] = p[i0 + f * threads];
+                if (i0 + f * threads < split.mine) {
+                    if constexpr (LAST) reinterpret_cast<int4 &>(raw[f]) = __ldcs(reinterpret_cast<const int4 *>(p + i0 + f * threads));
+                    else raw[f] = p[i0 + f * threads];
+                }
 #pragma unroll
             for (int f = 0; f < kInFlight; ++f) {
                 if (i0 + f * threads >= split.mine) break;
@@ -324,9 +318,12 @@ template <class T, class I> struct RowPart {
 // A cluster of 1 to 8 blocks takes a row: every block streams its part (largest value and sum of exponentials, both per
 // thread), the blocks exchange their sums through distributed shared memory, and (GRAD) read their parts again,
 // from the second-level cache, for the gradient: the logits cross the memory once.  The clusters that run at a
-// time hold 30 to 60 MB, which the cache keeps.  4096 x 128000 float16 takes 426 us (0.73 of the copy rate); the
+// time hold 30 to 60 MB, which the cache keeps.  4096 x 128000 float16 takes 400 us (0.80 of the copy rate); the
 // parts kept in shared memory instead, by copies that run ahead, 487 us, because few threads fit beside them; clusters
-// that stay and fetch the next row's teacher ahead, 766 us, because they read and write in step.
+// that stay and fetch the next row's teacher ahead, 766 us, because they read and write in step.  What a block waits for
+// beside its part counts as much as the bytes: the first logits are fetched with the teacher's entries, the student's
+// logits at their columns arrive while the part is streamed, and one warp forms the probabilities and the loss while the
+// others go on (418 us with these one after the other; 1024 x 150001 float32: 288, now 264).
 //
 // Two exponentials an element: at float16 and the copy rate that is 3.3e12 a second, three quarters of what the
 // special function units give; the rest of the arithmetic is done in pairs to stay out of their way.
@@ -343,14 +340,21 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
     constexpr int VEC = Part::VEC;
     extern __shared__ __align__(16) char shared_bytes[];
     __shared__ Sum warp_sums[kThreads / 32], rank_sums[kMaxRanks];
-    __shared__ A buf[kThreads / 32];
-    __shared__ int used;
     cudaGridDependencySynchronize();
     const uint32_t r = share.row();
     const int rank = share.rank(), ranks = 1 << share.bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x;
     const Part part(z + zm(r), vocab, k, share, shared_bytes);
     T *out = GRAD ? dz + dm(r) : nullptr;
-    if (!part.read_teacher(top + int64_t(r) * k, index + int64_t(r) * k, used)) {   // every block of the cluster
+    const V *from = part.from();
+    V raw[kInFlight], low;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) low.v[j] = from_acc<T>(A(-INFINITY));
+    const auto load = [&](int i0) {
+#pragma unroll
+        for (int f = 0; f < kInFlight; ++f) raw[f] = i0 + f * threads < part.split.mine ? from[i0 + f * threads] : low;
+    };
+    load(threadIdx.x);   // while the teacher's entries are on their way
+    if (!part.teacher.read(top + int64_t(r) * k, index + int64_t(r) * k, k, vocab)) {   // every block of the cluster
         if (rank == 0 && threadIdx.x == 0) {
             if (loss) loss[r] = 0;
             if (stats) stats[2 * int64_t(r)] = stats[2 * int64_t(r) + 1] = 0;
@@ -360,16 +364,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
     }
     // (waited for before the first write into another block's memory: that block has to have begun)
     if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const T student = part.student(threadIdx.x, rank == 0);
     const A alone = part.single >= 0 ? to_acc<A>(part.row[part.single]) : A(-INFINITY);
     Sum s = {alone, part.single >= 0 ? Exponent<T, FUSED>(alone, exp_scale).template exp<true>(alone) : A(0)};
-    const V *from = part.from();
-    V low;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) low.v[j] = from_acc<T>(A(-INFINITY));
     for (int i0 = threadIdx.x; i0 < part.split.mine; i0 += kInFlight * threads) {
-        V raw[kInFlight];
-#pragma unroll
-        for (int f = 0; f < kInFlight; ++f) raw[f] = i0 + f * threads < part.split.mine ? from[i0 + f * threads] : low;
         A best = largest<T, VEC>(raw[0]);
 #pragma unroll
         for (int f = 1; f < kInFlight; ++f) best = max_nan(best, largest<T, VEC>(raw[f]));
@@ -384,9 +382,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
             v.sum_into(sum);
         }
         s.sum += Values<A, VEC>::join(sum);
+        load(i0 + kInFlight * threads);
     }
-    part.read_at_teacher(rank == 0);
-    if (warp == 0) part.teacher.normalize(k, inv_temp);
+    // before any block writes over the logits
+    if (threadIdx.x < k) part.at_teacher[threadIdx.x] = to_acc<A>(student);
+    for (int i = threadIdx.x + threads; i < k; i += threads) part.at_teacher[i] = to_acc<A>(part.student(i, rank == 0));
     // lanes, warps and ranks, each in a fixed order
     s = s.over_warp(exp_scale);
     if (lane == 0) warp_sums[warp] = s;
@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
     s = s.over_warp(exp_scale);
     if (ranks > 1) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        // every rank writes its sum to every rank; the barrier of the cluster makes them visible (and follows the reads
-        // of read_at_teacher)
+        // every rank writes its sum to every rank; the barrier of the cluster makes them visible (and follows the
+        // reads of the student's logits)
         if (threadIdx.x < ranks) {
             const uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(&rank_sums[rank]));
             uint32_t remote;
@@ -411,17 +411,20 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
         s = lane < ranks ? rank_sums[lane] : Sum{-INFINITY, 0};
         s = s.over_warp(exp_scale);
     }
-    if (rank == 0) {
+    if (warp == 0) {   // the other warps go on
+        part.teacher.normalize(k, inv_temp);
         const A log_sum = s.log_sum(exp_scale);
         A total = 0;
-        for (int i = threadIdx.x; i < k; i += blockDim.x) {
-            if (part.teacher.at[i] < 0 || part.teacher.p[i] == 0) continue;
-            const A v = part.at_teacher[i];
-            total += part.teacher.p[i] *
-                     (part.teacher.logp[i] - (v == -INFINITY ? A(-INFINITY) : (v - s.top) * inv_temp - log_sum));
+        if (rank == 0) {
+            for (int i = lane; i < k; i += 32) {
+                if (part.teacher.at[i] < 0 || part.teacher.p[i] == 0) continue;
+                const A v = part.at_teacher[i];
+                total += part.teacher.p[i] *
+                         (part.teacher.logp[i] - (v == -INFINITY ? A(-INFINITY) : (v - s.top) * inv_temp - log_sum));
+            }
+            total = warp_fold(SumF(), total);
         }
-        total = block_fold(SumF(), total, buf);
-        if (threadIdx.x == 0) {
+        if (rank == 0 && lane == 0) {
             if (loss) loss[r] = temp * temp * total;
             if (stats) {
                 stats[2 * int64_t(r)] = s.top;
@@ -431,7 +434,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
     }
     if constexpr (GRAD) {
         const RowGradient<T, FUSED> grad(s, exp_scale, dloss[r * dstep] * temp);
-        part.dense_gradient(out, grad);
+        if (part.on_lines()) part.template dense_gradient<true>(out, grad);
+        else part.template dense_gradient<false>(out, grad);
         __syncthreads();
         part.teacher_gradient(out, grad);
     }
@@ -447,16 +451,15 @@ __global__ void __launch_bounds__(kThreads)
 {
     using A = acc_t<T>;
     extern __shared__ __align__(16) char shared_bytes[];
-    __shared__ int used;
     cudaGridDependencySynchronize();
     const uint32_t r = share.row();
     const RowPart<T, I> part(z + zm(r), vocab, k, share, shared_bytes);
     T *out = dz + dm(r);
-    if (!part.read_teacher(top + int64_t(r) * k, index + int64_t(r) * k, used)) return part.zeros(out);
-    part.read_at_teacher(false);
+    if (!part.teacher.read(top + int64_t(r) * k, index + int64_t(r) * k, k, vocab)) return part.zeros(out);
+    for (int i = threadIdx.x; i < k; i += blockDim.x) part.at_teacher[i] = to_acc<A>(part.student(i, false));
     __syncthreads();
     const RowGradient<T, FUSED> grad(stats[2 * int64_t(r)], stats[2 * int64_t(r) + 1], exp_scale, dloss[r * dstep] * temp);
-    part.dense_gradient(out, grad);
+    part.template dense_gradient<false>(out, grad);
     if (threadIdx.x < 32) part.teacher.normalize(k, inv_temp);
     __syncthreads();
     part.teacher_gradient(out, grad);
@@ -512,10 +515,10 @@ template <class T, class I, bool GRAD, bool FUSED> static int run_rows(const Dis
 {
     using A = acc_t<T>;
     Shares share;
-    // 4096 x 128000 float16: loss 186 us with whole rows of 250 KiB, 195 with halves, 238 with quarters; loss and
-    // gradient 421 with quarters, 477 with halves (what the clusters hold has to stay in the cache between the
-    // two readings)
-    DPB_TRY(share_row(a, sizeof(T), (GRAD ? 64 : 256) * 1024, 3, share));
+    // Loss: whole rows (4096 x 128000 float16: 181 us, 185 with halves, 212 with quarters; 8192 x 150001 float32: 715 us,
+    // 900 with quarters).  Loss and gradient: what the clusters hold has to stay in the cache between the two readings
+    // (4096 x 128000 float16: 400 us with quarters, 476 with halves).
+    DPB_TRY(share_row(a, sizeof(T), GRAD ? 64 * 1024 : INT64_MAX, 3, share));
     launch_cluster(distillation_row_kernel<T, I, GRAD, FUSED>, static_cast<unsigned>(a.rows << share.bits), 1u << share.bits, share_threads(share),
                    RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const T *>(a.z->data), a.zm,
                    static_cast<const A *>(a.top->data), static_cast<const I *>(a.index->data), static_cast<int>(a.k),

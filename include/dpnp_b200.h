@@ -519,7 +519,7 @@ int dpb_embedding_backward(const dpb_array *dout, const dpb_array *ids, double s
 /* Distillation.  logits: rows of V; teacher_logits (accumulation type) and teacher_index (int32 or int64):
  * C-contiguous rows of K <= 1024 entries.  An entry counts when its index lies in [0, V) and its logit is
  * above -inf; p = softmax(teacher_logits / T) over those, q = softmax(logits / T);
- * loss = T^2 * sum p (log p - log q), 0 for a row without entries, whose logits are not read.
+ * loss = T^2 * sum p (log p - log q), 0 for a row without entries.
  * stats (NULL, or shape of the rows + (2,), accumulation type): max of the row's logits and
  * log sum exp((logits - max) / T), zeros for a row without entries. */
 int dpb_distillation_loss(const dpb_array *logits, const dpb_array *teacher_logits, const dpb_array *teacher_index,

@@ -719,6 +719,26 @@ def test_distillation_layouts_and_in_place(dt, vocab):
     assert np.array_equal(host(big)[:, 5:vocab + 5], want) and (host(big)[:, :5] == 3).all() and (host(big)[:, vocab + 5:] == 3).all()
 
 
+@pytest.mark.parametrize("rows,vocab,k", [(9, 512, 300), (40, 65536, 12), (700, 32832, 40), (3, 131072, 600)])
+@pytest.mark.parametrize("dt", TYPES)
+def test_distillation_in_place_on_cache_lines(dt, rows, vocab, k):
+    """Rows of whole lines that several blocks share, more entries than threads, rows without entries that hold NaN."""
+    import dpnp_b200 as dp
+
+    if dt == "f8":
+        rows = min(rows, 12)
+    z, t, idx, rng = distil_data(rows, vocab, k, dt, vocab + k)
+    idx[::3] = -1
+    z[::3] = np.nan
+    g = rng.uniform(0.5, 2, rows).astype(ACC[dt])
+    over = dev(z)
+    loss, grad = dp.distillation_loss_and_grad(over, dev(t), dev(idx), dev(g), temperature=1.5, out=(None, over))
+    assert grad is over
+    check_distil(z, t, idx, 1.5, host(loss), host(grad), None, g)
+    again = dp.distillation_loss_and_grad(dev(z), dev(t), dev(idx), dev(g), temperature=1.5)
+    assert np.array_equal(host(again[0]), host(loss)) and np.array_equal(host(again[1]), host(grad))
+
+
 def test_distillation_gradient_against_differences():
     """float64, central differences of the summed losses (bounds as for the layer norm)."""
     import dpnp_b200 as dp
