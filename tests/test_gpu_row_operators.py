@@ -153,6 +153,14 @@ def test_layer_norm_rows_off_the_vector_grid(dt, rows, n, pad):
     assert not host(buf)[:1].any() and not host(buf)[rows * n + 4:].any()
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,n,pad", [(2600, 523, 0), (2600, 305, 2), (2600, 151, 1), (900, 4099, 0), (601, 9001, 0), (450, 12003, 1),
+                                        (301, 16001, 3), (160, 32011, 0)])
+def test_layer_norm_rows_off_the_vector_grid_in_other_forms(dt, rows, n, pad):
+    """The widths at which the forward kernel's threads, accesses and places of the weights change."""
+    test_layer_norm_rows_off_the_vector_grid(dt, rows, n, pad)
+
+
 def check_norm_backward(x, dy, w, mean, rstd, dx, dw, db):
     dt = x.dtype.str[1:]
     wide, u, n = WIDE[dt], unit(dt), x.shape[-1]
