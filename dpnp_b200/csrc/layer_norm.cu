@@ -636,6 +636,8 @@ static int launch_backward(const NormGradArgs &a, int64_t accesses, cudaStream_t
 //   512 threads an SM, two accesses, one row: 95 / 82; two rows: 96 / 74 (92 / 74 at 2048 columns).
 // More accesses a thread cost fewer instructions around the folds, fewer threads leave 128 registers for the
 // accumulators.  Shifted rows of float16 need registers for the edges too: one row, 640 threads.
+// Shifted rows of other types just above 1024 accesses take four, so that two blocks fit an SM (16380 x 4097 float32: 173
+// us against 240 with one block of 544 threads; at 6001 columns that form is slower, 226 against 197).
 // False: the row is too long (then the columns are summed by a second pass over dy and x).
 template <class T, class W, int VEC, bool SHIFT> static bool run_rows_backward(const NormGradArgs &a, cudaStream_t s, int &st)
 {
@@ -659,6 +661,9 @@ template <class T, class W, int VEC, bool SHIFT> static bool run_rows_backward(c
         }
         else {
             DPB_BACK(1024, 2, false, 2, 2, false, 512)
+        }
+        if constexpr (SHIFT && !is_half_v<T>) {
+            DPB_BACK(1280, 4, false, 1, 2, false, 640)
         }
         if constexpr (SHIFT) {
             DPB_BACK(2048, 2, false, 1, 2, false, 1024)
