@@ -580,7 +580,7 @@ template <class T, class W> static int run_forward(const NormArgs &a, cudaStream
     const bool aligned = row_vector(a.x->data, a.xm, a.n, sizeof(T), wide) == wide &&
                          row_vector(a.y->data, a.ym, a.n, sizeof(T), wide) == wide && wide_ok(w, wide, sizeof(W)) &&
                          wide_ok(b, wide, sizeof(W));
-    const bool shifted = a.xm.outer == 0 || a.rows == 1;
+    const bool shifted = a.xm.one_stride();
     if (aligned ? run_rows<T, W, wide, false>(a, s)
                 : shifted ? run_rows<T, W, wide, true>(a, s) : run_rows<T, W, 1, false>(a, s)) {
         note_kernel("layer_norm");
@@ -688,7 +688,7 @@ template <class T, class W> static int run_backward(const NormGradArgs &a, cudaS
                              row_vector(dy, a.dym, a.n, sizeof(T), wide) == wide &&
                              row_vector(a.dx->data, a.dxm, a.n, sizeof(T), wide) == wide;
         // shifted columns: rows one stride apart that start at the same misalignment in dy and x
-        const bool shifted = (a.rows == 1 || (a.xm.outer == 0 && a.dym.outer == 0 && (a.xm.inner - a.dym.inner) % wide == 0)) &&
+        const bool shifted = (a.rows == 1 || (a.xm.one_stride() && a.dym.one_stride() && (a.xm.inner - a.dym.inner) % wide == 0)) &&
                              (reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(dy)) % 16 == 0;
         int st = DPB_OK;
         if (aligned ? run_rows_backward<T, W, wide, false>(a, s, st)

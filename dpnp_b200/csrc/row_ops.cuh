@@ -34,7 +34,9 @@ template <class T, class A> DPB_D T from_acc(A v)
 struct RowMap {
     int64_t outer, inner;   // strides of the two levels in elements
     FastDiv32 extent;       // rows of one inner level
-    DPB_D int64_t operator()(uint32_t r) const
+    bool nested = false;    // two levels (whatever their strides are: an outer one of 0 is a broadcast axis)
+    DPB_HD bool one_stride() const { return !nested; }   // all rows are `inner` apart
+    DPB_HD int64_t operator()(uint32_t r) const
     {
         uint32_t q, m;
         extent.divmod(r, q, m);
@@ -47,13 +49,13 @@ template <class T> struct RowWalk {
     T *base, *p;
     RowMap map;
     int64_t delta;
-    DPB_D RowWalk(T *data, const RowMap &m, uint32_t r, uint32_t step)
-        : base(data), p(data + m(r)), map(m), delta(m.outer == 0 ? int64_t(step) * m.inner : 0)
+    DPB_HD RowWalk(T *data, const RowMap &m, uint32_t r, uint32_t step)
+        : base(data), p(data + m(r)), map(m), delta(m.one_stride() ? int64_t(step) * m.inner : 0)
     {
     }
-    DPB_D void next(uint32_t r)   // to row r, one step on (r < 2^31: the caller does not go beyond the last row)
+    DPB_HD void next(uint32_t r)   // to row r, one step on (r < 2^31: the caller does not go beyond the last row)
     {
-        if (map.outer == 0) p += delta;
+        if (map.one_stride()) p += delta;
         else p = base + map(r);
     }
 };
@@ -79,7 +81,8 @@ inline bool make_row_map(const dpb_array &a, RowMap &map)
         str[levels] = st[i];
         ++levels;
     }
-    if (levels == 2) {
+    map.nested = levels == 2;
+    if (map.nested) {
         map.outer = str[0];
         map.inner = str[1];
         map.extent = FastDiv32(static_cast<uint32_t>(ext[1]));

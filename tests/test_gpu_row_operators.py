@@ -950,3 +950,88 @@ def test_writes_stay_inside_the_results():
         assert report() == (0, 0)
     finally:
         check(lib.dpb_set_tuning(b"redzones", 0))
+
+
+# ------------------------------------------------------------- rows in two levels, more of them than groups of threads
+def _two_levels(dp, kind, base):
+    """An array (B, S, n) of rows in two levels, on the GPU and as NumPy sees it; `base` is (B, S + 3, n + 8)."""
+    d, n, s = dev(base), base.shape[2] - 8, base.shape[1] - 3
+    shape = (base.shape[0], s, n)
+    if kind == "broadcast":                            # one matrix for all of the leading axis
+        return dp.broadcast_to(d[0, :s, :n], shape), np.broadcast_to(base[0, :s, :n], shape)
+    if kind == "broadcast, shifted":
+        return dp.broadcast_to(d[0, 1:s + 1, 1:n + 1], shape), np.broadcast_to(base[0, 1:s + 1, 1:n + 1], shape)
+    if kind == "broadcast inner":                      # one row for all of the inner axis
+        return dp.broadcast_to(d[:, :1, :n], shape), np.broadcast_to(base[:, :1, :n], shape)
+    return d[:, 2:s + 2, 8:], base[:, 2:s + 2, 8:]     # a slice: two different strides
+
+
+TWO_LEVELS = ["broadcast", "broadcast, shifted", "broadcast inner", "slice"]
+# (more rows than groups of threads that the GPU holds: a warp a row, then one to thirty-two warps a row)
+MANY_ROWS = [(40, 130, 96), (43, 127, 37), (4, 330, 2048), (6, 301, 1001), (4, 90, 8192), (5, 70, 5001), (3, 20, 40000)]
+
+
+@pytest.mark.parametrize("b,s,n", MANY_ROWS)
+@pytest.mark.parametrize("kind", TWO_LEVELS)
+@pytest.mark.parametrize("dt,wt", NORM_TYPES)
+def test_layer_norm_of_rows_in_two_levels(dt, wt, kind, b, s, n):
+    import dpnp_b200 as dp
+
+    if dt == "f8" and n > 1000:
+        b = max(2, b // 2)
+    rng = np.random.default_rng(b * s + n)
+    base = (rng.normal(0, 1, (b, s + 3, n + 8)) + rng.normal(0, 2, (b, s + 3, 1))).astype(dt)
+    w, bias = (1 + 0.3 * rng.normal(0, 1, n)).astype(wt), (0.3 * rng.normal(0, 1, n)).astype(wt)
+    d, x = _two_levels(dp, kind, base)
+    dense = np.ascontiguousarray(x)
+    y, mean, rstd = dp.layer_norm(d, dev(w), dev(bias), return_stats=True)
+    check_norm(dense, w, bias, 1e-5, host(y), host(mean), host(rstd))
+    big = dp.zeros(base.shape, dtype=dt)               # a result whose rows are in two levels
+    dp.layer_norm(dev(dense), dev(w), dev(bias), out=big[:, 1:s + 1, 3:n + 3])
+    got = host(big)
+    check_norm(dense, w, bias, 1e-5, got[:, 1:s + 1, 3:n + 3], host(mean), host(rstd))
+    got[:, 1:s + 1, 3:n + 3] = 0
+    assert not got.any()
+
+
+@pytest.mark.parametrize("b,s,n", MANY_ROWS)
+@pytest.mark.parametrize("kind", TWO_LEVELS)
+@pytest.mark.parametrize("dt,wt", NORM_TYPES)
+def test_layer_norm_backward_of_rows_in_two_levels(dt, wt, kind, b, s, n):
+    """x and dy in two levels, one after the other and both."""
+    import dpnp_b200 as dp
+
+    if dt == "f8" and n > 1000:
+        b = max(2, b // 2)
+    rng = np.random.default_rng(b * s + n)
+    base = rng.normal(0, 1, (2, b, s + 3, n + 8)).astype(dt)
+    w = (1 + 0.3 * rng.normal(0, 1, n)).astype(wt)
+    (dx_, x), (dg, g) = (_two_levels(dp, kind, base[i]) for i in range(2))
+    xc, gc = np.ascontiguousarray(x), np.ascontiguousarray(g)
+    _, mean, rstd = dp.layer_norm(dev(xc), return_stats=True)
+    m, r = host(mean), host(rstd)
+    for dy, at in ((dg, dev(xc)), (dev(gc), dx_), (dg, dx_)):
+        out = dp.layer_norm_backward(dy, at, mean, rstd, dev(w))
+        check_norm_backward(xc, gc, w, m, r, *map(host, out))
+    big = dp.zeros(base.shape[1:], dtype=dt)
+    dp.layer_norm_backward(dg, dx_, mean, rstd, dev(w), out=(big[:, 1:s + 1, 3:n + 3], None, None))
+    check_norm_backward(xc, gc, w, m, r, host(big)[:, 1:s + 1, 3:n + 3], None, None)
+
+
+@pytest.mark.parametrize("kind", TWO_LEVELS)
+@pytest.mark.parametrize("dt", TYPES)
+def test_embedding_and_distillation_of_rows_in_two_levels(dt, kind):
+    import dpnp_b200 as dp
+
+    rng = np.random.default_rng(12)
+    b, s, n = 30, 101, 75
+    d, x = _two_levels(dp, kind, rng.normal(0, 2, (b, s + 3, n + 8)).astype(dt))
+    x = np.ascontiguousarray(x)
+    ids = rng.integers(-1, 60, (b, s)).astype("i4")
+    check_embedding_backward(x, ids, 60, 0.5, host(dp.embedding_backward(d, dev(ids), 60, scale=0.5)), dt)
+    t, idx = rng.normal(0, 2, (b, s, 4)).astype(ACC[dt]), rng.integers(-1, n, (b, s, 4)).astype("i4")
+    loss, stats = dp.distillation_loss(d, dev(t), dev(idx), return_stats=True)
+    check_distil(x, t, idx, 1.0, host(loss), None, host(stats))
+    check_distil(x, t, idx, 1.0, None, host(dp.distillation_loss_backward(1.0, d, dev(t), dev(idx), stats)))
+    loss, grad = dp.distillation_loss_and_grad(d, dev(t), dev(idx))
+    check_distil(x, t, idx, 1.0, host(loss), host(grad))
