@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(WARP ? 256 : THREADS, WARP ? THREADS / 256 : 1
         const auto load = [&](int k, int i, Vals &aa, Vals &hh) {
             unpack<A, VEC, T>(slot[((turn * R + k) * 2 * ITEMS + i) * threads], aa);
             unpack<A, VEC, T>(slot[(((turn * R + k) * 2 + 1) * ITEMS + i) * threads], hh);
-            hh.add(-m[k]);
+            hh.add(at.any(i) ? -m[k] : A(0));   // zeros outside the row stay zeros (m rs may be infinite)
             hh.mul(rs[k]);
             if (SHIFT && edge[i]) {
                 at.clip(i, aa);
@@ -636,7 +636,7 @@ static int launch_backward(const NormGradArgs &a, int64_t accesses, cudaStream_t
 //   512 threads an SM, two accesses, one row: 95 / 82; two rows: 96 / 74 (92 / 74 at 2048 columns).
 // More accesses a thread cost fewer instructions around the folds, fewer threads leave 128 registers for the
 // accumulators.  Shifted rows of float16 need registers for the edges too: one row, 640 threads.
-// Shifted rows of other types just above 1024 accesses take four, so that two blocks fit an SM (16380 x 4097 float32: 173
+// Shifted rows of other types just above 1024 accesses take four, so that two blocks fit an SM (16380 x 4097 float32: 156
 // us against 240 with one block of 544 threads; at 6001 columns that form is slower, 226 against 197).
 // False: the row is too long (then the columns are summed by a second pass over dy and x).
 template <class T, class W, int VEC, bool SHIFT> static bool run_rows_backward(const NormGradArgs &a, cudaStream_t s, int &st)

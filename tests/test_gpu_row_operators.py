@@ -1035,3 +1035,23 @@ def test_embedding_and_distillation_of_rows_in_two_levels(dt, kind):
     check_distil(x, t, idx, 1.0, None, host(dp.distillation_loss_backward(1.0, d, dev(t), dev(idx), stats)))
     loss, grad = dp.distillation_loss_and_grad(d, dev(t), dev(idx))
     check_distil(x, t, idx, 1.0, host(loss), host(grad))
+
+
+@pytest.mark.parametrize("n", [1, 60, 64, 100, 256, 1000, 1024, 1537, 4100, 8192, 70001])
+@pytest.mark.parametrize("dt", ["f4", "f8"])
+def test_layer_norm_backward_of_constant_rows_of_large_values(dt, n):
+    """x - mean is 0 there, and so is h, although mean * rstd is beyond the type's range: nothing of that product may
+    come into the sums from threads that have no column."""
+    import dpnp_b200 as dp
+
+    rng = np.random.default_rng(n)
+    rows, big = 9, 2.0**(123 if dt == "f4" else 1019)
+    x = np.broadcast_to(big * (-1.0)**np.arange(rows)[:, None], (rows, n)).astype(dt)
+    mean, rstd = np.ascontiguousarray(x[:, 0]), np.full(rows, 316.0, dt)
+    assert 316.0 * big > float(np.finfo(dt).max)
+    w, dy = (1 + 0.3 * rng.normal(0, 1, n)).astype(dt), rng.normal(0, 1, (rows, n)).astype(dt)
+    for pad in (0, 1):                                 # rows on the 16-byte grid, and off it
+        wide = np.zeros((2, rows, n + pad), dt)
+        wide[0, :, pad:], wide[1, :, pad:] = dy, x
+        out = dp.layer_norm_backward(dev(wide[0])[:, pad:], dev(wide[1])[:, pad:], dev(mean), dev(rstd), dev(w))
+        check_norm_backward(x, dy, w, mean, rstd, *map(host, out))
