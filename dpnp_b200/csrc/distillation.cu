@@ -502,11 +502,12 @@ template <class T, class I, bool FUSED> static int run_grad(const DistilArgs &a,
     // parts of 64 to 128 KiB: below that the teacher's entries, which every block reads, show (1024 x 150001 float32:
     // 221 us at 75 KiB, 266 us at 37 KiB)
     DPB_TRY(share_row(a, sizeof(T), 128 * 1024, 10, share));
-    launch_shared(distillation_grad_kernel<T, I, FUSED>, static_cast<unsigned>(a.rows << share.bits), share_threads(share),
-                  RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const A *>(a.dloss->data), a.dloss->nd == 0 ? 0 : 1,
-                  static_cast<const T *>(a.z->data), a.zm, static_cast<const A *>(a.top->data),
-                  static_cast<const I *>(a.index->data), static_cast<int>(a.k), static_cast<int>(a.vocab), A(a.temp),
-                  A(1.0 / a.temp), A(kLog2E / a.temp), static_cast<const A *>(a.stats->data), static_cast<T *>(a.dz->data), a.dm, share);
+    launch_shared<distillation_grad_kernel<T, I, FUSED>>(
+        static_cast<unsigned>(a.rows << share.bits), share_threads(share), RowPart<T, I>::shared_bytes(int(a.k)), s,
+        static_cast<const A *>(a.dloss->data), a.dloss->nd == 0 ? 0 : 1, static_cast<const T *>(a.z->data), a.zm,
+        static_cast<const A *>(a.top->data), static_cast<const I *>(a.index->data), static_cast<int>(a.k),
+        static_cast<int>(a.vocab), A(a.temp), A(1.0 / a.temp), A(kLog2E / a.temp), static_cast<const A *>(a.stats->data),
+        static_cast<T *>(a.dz->data), a.dm, share);
     note_kernel("distillation_grad");
     return check_launch("distillation_grad");
 }
@@ -519,13 +520,14 @@ template <class T, class I, bool GRAD, bool FUSED> static int run_rows(const Dis
     // 900 with quarters).  Loss and gradient: what the clusters hold has to stay in the cache between the two readings
     // (4096 x 128000 float16: 400 us with quarters, 476 with halves).
     DPB_TRY(share_row(a, sizeof(T), GRAD ? 64 * 1024 : INT64_MAX, 3, share));
-    launch_cluster(distillation_row_kernel<T, I, GRAD, FUSED>, static_cast<unsigned>(a.rows << share.bits), 1u << share.bits, share_threads(share),
-                   RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const T *>(a.z->data), a.zm,
-                   static_cast<const A *>(a.top->data), static_cast<const I *>(a.index->data), static_cast<int>(a.k),
-                   static_cast<int>(a.vocab), A(a.temp), A(1.0 / a.temp), A(kLog2E / a.temp),
-                   a.loss ? static_cast<A *>(a.loss->data) : nullptr, a.stats ? static_cast<A *>(a.stats->data) : nullptr,
-                   GRAD ? static_cast<const A *>(a.dloss->data) : nullptr, GRAD && a.dloss->nd > 0 ? 1 : 0,
-                   GRAD ? static_cast<T *>(a.dz->data) : nullptr, a.dm, share);
+    launch_cluster<distillation_row_kernel<T, I, GRAD, FUSED>>(
+        static_cast<unsigned>(a.rows << share.bits), 1u << share.bits, share_threads(share),
+        RowPart<T, I>::shared_bytes(int(a.k)), s, static_cast<const T *>(a.z->data), a.zm,
+        static_cast<const A *>(a.top->data), static_cast<const I *>(a.index->data), static_cast<int>(a.k),
+        static_cast<int>(a.vocab), A(a.temp), A(1.0 / a.temp), A(kLog2E / a.temp),
+        a.loss ? static_cast<A *>(a.loss->data) : nullptr, a.stats ? static_cast<A *>(a.stats->data) : nullptr,
+        GRAD ? static_cast<const A *>(a.dloss->data) : nullptr, GRAD && a.dloss->nd > 0 ? 1 : 0,
+        GRAD ? static_cast<T *>(a.dz->data) : nullptr, a.dm, share);
     note_kernel("distillation_row");
     return check_launch("distillation_row");
 }

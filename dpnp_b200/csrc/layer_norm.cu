@@ -534,11 +534,12 @@ static bool launch_forward(const NormArgs &a, int64_t accesses, cudaStream_t s)
     const int groups = WARP ? 8 : 1, threads = WARP ? 256 : static_cast<int>(ceil_div(ceil_div(accesses, ITEMS), 32) * 32);
     const size_t shared = size_t(DEPTH) * R * ITEMS * threads * sizeof(T) * VEC +
                           (KEEP == kShared ? KeptWeights<W, VEC, ITEMS>::bytes(threads) : 0);
-    launch_shared(layer_norm_kernel<T, W, VEC, ITEMS, WARP, R, DEPTH, KEEP, SHIFT>, block_count(a.rows, groups, 1, threads, shared, SHIFT, kGroupThreads),
-                  unsigned(threads), shared, s, static_cast<const T *>(a.x->data), a.xm, row_neighbours<T>(*a.x, *a.y),
-                  a.w ? static_cast<const W *>(a.w->data) : nullptr, a.b ? static_cast<const W *>(a.b->data) : nullptr,
-                  A(a.eps), static_cast<T *>(a.y->data), a.ym, a.mean ? static_cast<A *>(a.mean->data) : nullptr,
-                  a.rstd ? static_cast<A *>(a.rstd->data) : nullptr, static_cast<uint32_t>(a.rows), static_cast<int>(a.n));
+    launch_shared<layer_norm_kernel<T, W, VEC, ITEMS, WARP, R, DEPTH, KEEP, SHIFT>>(
+        block_count(a.rows, groups, 1, threads, shared, SHIFT, kGroupThreads), unsigned(threads), shared, s,
+        static_cast<const T *>(a.x->data), a.xm, row_neighbours<T>(*a.x, *a.y),
+        a.w ? static_cast<const W *>(a.w->data) : nullptr, a.b ? static_cast<const W *>(a.b->data) : nullptr, A(a.eps),
+        static_cast<T *>(a.y->data), a.ym, a.mean ? static_cast<A *>(a.mean->data) : nullptr,
+        a.rstd ? static_cast<A *>(a.rstd->data) : nullptr, static_cast<uint32_t>(a.rows), static_cast<int>(a.n));
     return true;
 }
 
@@ -617,11 +618,11 @@ static int launch_backward(const NormGradArgs &a, int64_t accesses, cudaStream_t
     const unsigned blocks = block_count(a.rows, groups, R, threads, shared, SHIFT, THREADS);
     void *part = nullptr;
     if (a.dw) DPB_TRY(dpb_malloc(static_cast<size_t>(int64_t(blocks) * 2 * a.n) * sizeof(A), s, &part));
-    launch_shared(layer_norm_backward_kernel<T, W, VEC, ITEMS, WARP, R, DEPTH, HOLD, SHIFT, THREADS>, blocks, unsigned(threads), shared, s,
-                  static_cast<const T *>(a.dy->data), a.dym, row_neighbours<T>(*a.dy, *a.dx),
-                  static_cast<const T *>(a.x->data), a.xm, row_neighbours<T>(*a.x, *a.dx), static_cast<const A *>(a.mean->data),
-                  static_cast<const A *>(a.rstd->data), a.w ? static_cast<const W *>(a.w->data) : nullptr,
-                  static_cast<T *>(a.dx->data), a.dxm, static_cast<A *>(part), static_cast<uint32_t>(a.rows), static_cast<int>(a.n));
+    launch_shared<layer_norm_backward_kernel<T, W, VEC, ITEMS, WARP, R, DEPTH, HOLD, SHIFT, THREADS>>(
+        blocks, unsigned(threads), shared, s, static_cast<const T *>(a.dy->data), a.dym, row_neighbours<T>(*a.dy, *a.dx),
+        static_cast<const T *>(a.x->data), a.xm, row_neighbours<T>(*a.x, *a.dx), static_cast<const A *>(a.mean->data),
+        static_cast<const A *>(a.rstd->data), a.w ? static_cast<const W *>(a.w->data) : nullptr,
+        static_cast<T *>(a.dx->data), a.dxm, static_cast<A *>(part), static_cast<uint32_t>(a.rows), static_cast<int>(a.n));
     note_kernel("layer_norm_backward");
     int st = check_launch("layer_norm_backward");
     if (part) {

@@ -3,6 +3,7 @@
 // checks of their entry points.
 #pragma once
 
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
 #include <vector>
@@ -111,13 +112,36 @@ inline bool wide_ok(const void *p, int vec, int item)
     return !p || is_aligned(p, static_cast<size_t>(bytes > 16 ? 16 : bytes));
 }
 
-// launch_after_previous with dynamic shared memory (a block of more than 48 KiB in all has to ask for it) and
-// clusters of `cluster` blocks.
-template <class... KArgs, class... Args>
-inline void launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned cluster, unsigned block, size_t shared,
-                           cudaStream_t stream, Args... args)
+// Lets a kernel have as much dynamic shared memory as a block can (more than 48 KiB in all have to be asked for).  The limit
+// belongs to the function on the device and all threads of the program share it: it is raised once and stays, because a
+// limit set to each call's own size could be lowered by another thread before the launch.  False: an error, which is left in
+// cudaGetLastError.
+template <auto kernel> inline bool allow_shared()
 {
-    if (shared > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
+    static std::atomic<uint64_t> done{0};   // a bit a device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return true;
+    cudaFuncAttributes has;
+    if (cudaFuncGetAttributes(&has, kernel) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             device_props().max_smem_optin - static_cast<int>(has.sharedSizeBytes)) != cudaSuccess)
+        return false;
+    if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+    return true;
+}
+
+template <class... KArgs, class... Args> inline void launch_config(const cudaLaunchConfig_t &cfg, void (*kernel)(KArgs...), Args... args)
+{
+    cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);   // an error stays in cudaGetLastError for check_launch
+}
+
+// launch_after_previous with dynamic shared memory and clusters of `cluster` blocks.
+template <auto kernel, class... Args>
+inline void launch_cluster(unsigned grid, unsigned cluster, unsigned block, size_t shared, cudaStream_t stream, Args... args)
+{
+    if (shared > 40 * 1024 && !allow_shared<kernel>()) return;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
@@ -135,12 +159,12 @@ inline void launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned clu
         attr[cfg.numAttrs++].val.clusterDim.z = 1;
     }
     cfg.attrs = attr;
-    cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);   // an error stays in cudaGetLastError for check_launch
+    launch_config(cfg, kernel, args...);
 }
-template <class... KArgs, class... Args>
-inline void launch_shared(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t shared, cudaStream_t stream, Args... args)
+template <auto kernel, class... Args>
+inline void launch_shared(unsigned grid, unsigned block, size_t shared, cudaStream_t stream, Args... args)
 {
-    launch_cluster(kernel, grid, 1u, block, shared, stream, args...);
+    launch_cluster<kernel>(grid, 1u, block, shared, stream, args...);
 }
 
 // -------------------------------------------------------------------------------- argument checks

@@ -1055,3 +1055,57 @@ def test_layer_norm_backward_of_constant_rows_of_large_values(dt, n):
         wide[0, :, pad:], wide[1, :, pad:] = dy, x
         out = dp.layer_norm_backward(dev(wide[0])[:, pad:], dev(wide[1])[:, pad:], dev(mean), dev(rstd), dev(w))
         check_norm_backward(x, dy, w, mean, rstd, *map(host, out))
+
+
+def test_threads_with_rows_of_other_widths():
+    """Two host threads at once in the C entry points, with widths for which one and the same kernel takes different
+    amounts of shared memory: no call is refused, and the results are those of a single thread."""
+    import ctypes as C
+    import threading
+
+    import dpnp_b200 as dp
+    from dpnp_b200 import _lib
+
+    def job(n, seed):
+        q = dp.StreamQueue(0)
+        x, w, b, rng = norm_data(5, n, "f4", "f4", seed)
+        put = lambda a: dp.tensor.asarray(a, sycl_queue=q)  # noqa: E731
+        a = dict(x=put(x), w=put(w), b=put(b), dy=put(rng.normal(0, 1, x.shape).astype("f4")),
+                 **{k: put(np.zeros(x.shape, "f4")) for k in ("y", "dx")}, mean=put(np.zeros(5, "f4")), rstd=put(np.zeros(5, "f4")),
+                 **{k: put(np.zeros(n, "f4")) for k in ("dw", "db")})
+        keep = {k: v._descriptor() for k, v in a.items()}
+        at = {k: C.byref(d[0]) for k, d in keep.items()}
+        stream = C.c_void_p(q.stream)
+
+        def step():
+            return (_lib.lib.dpb_layer_norm(at["x"], at["w"], at["b"], 1e-5, at["y"], at["mean"], at["rstd"], stream),
+                    _lib.lib.dpb_layer_norm_backward(at["dy"], at["x"], at["mean"], at["rstd"], at["w"], at["dx"], at["dw"],
+                                                     at["db"], stream))
+
+        def results():
+            q.wait()
+            return [dp.tensor.asnumpy(a[k]) for k in ("y", "mean", "rstd", "dx", "dw", "db")]
+
+        return step, results, keep
+
+    # forward: 64 KiB and 44 KiB; backward: 80 KiB and 55 KiB
+    jobs = [job(8192, 1), job(5632, 2), job(4096, 3), job(2816, 4)]
+    want = []
+    for step, results, _ in jobs:
+        assert step() == (_lib.OK, _lib.OK)
+        want.append(results())
+    refused, start = [], threading.Barrier(len(jobs))
+
+    def loop(step):
+        start.wait()
+        for _ in range(3000):
+            refused.extend(s for s in step() if s != _lib.OK)
+
+    threads = [threading.Thread(target=loop, args=(step,)) for step, _, _ in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not refused
+    for (_, results, _), w in zip(jobs, want):
+        assert all(np.array_equal(p, q) for p, q in zip(results(), w))
