@@ -227,6 +227,8 @@ def _direct_layer_norm_backward(dy, x, mean, rstd, weight, weight_grads, out):
     outs = _outs(out, 3)
     if outs is None or type(x) is not usm_ndarray or not x._shape or not weight_grads:
         return None
+    if dy is None or mean is None or rstd is None:
+        return None
     q = x._queue
     if not _plain_rows(q, x, dy, outs[0]) or not _plain(q, mean, rstd, weight, *outs[1:]) or x._dtype not in _ACCUMULATION or x._shape[-1] == 0:
         return None
@@ -555,8 +557,9 @@ def _row_gradient(dloss, shape, acc, q):
             raise ValueError(f"dloss: expected shape {shape} or (), got {dloss._shape}")
         _accumulation_type(dloss, "dloss")
         return _typed(dloss, acc, q)
+    value = _number(dloss, "dloss")
     res = _empty((), acc, q)
-    ti._full_usm_ndarray(_number(dloss, "dloss"), res, q)
+    ti._full_usm_ndarray(value, res, q)
     return res
 
 

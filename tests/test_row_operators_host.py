@@ -215,3 +215,27 @@ def test_the_functions_are_public_in_both_layers():
     for name in ("layer_norm", "layer_norm_backward", "embedding", "embedding_backward", "distillation_loss",
                  "distillation_loss_backward", "distillation_loss_and_grad"):
         assert getattr(dp, name).__doc__ == getattr(dpt, name).__doc__ and getattr(dp, name).__doc__
+
+
+def _one_queue():
+    """Valid positional arguments of every operator, all on one queue object (the direct route)."""
+    q = memory.StreamQueue(0, stream=7)
+
+    def a(*shape, dt="f4"):
+        _at[0] += 1 << 30
+        return usm_ndarray._view(_Mem, _at[0], shape, tuple(_dense_strides(shape)), np.dtype(dt), q, True)
+
+    z, t, j = a(4, 50), a(4, 3), a(4, 3, dt="i4")
+    return {"layer_norm": [a(4, 8)], "layer_norm_backward": [a(4, 8), a(4, 8), a(4), a(4)], "embedding": [a(4, 8), a(3, dt="i4")],
+            "embedding_backward": [a(3, 8), a(3, dt="i4"), 10], "distillation_loss": [z, t, j],
+            "distillation_loss_backward": [a(4), z, t, j, a(4, 2)], "distillation_loss_and_grad": [z, t, j, a(4)]}
+
+
+@pytest.mark.parametrize("name", sorted(_one_queue()))
+@pytest.mark.parametrize("layer", [dp, dp.tensor])
+def test_a_required_argument_that_is_no_array_is_a_type_error(layer, name):
+    args = _one_queue()[name]
+    for i in range(len(args)):
+        for wrong in (None, "1", [1.0], np.ones((4, 8), "f4"), 1j):
+            with pytest.raises(TypeError):
+                getattr(layer, name)(*args[:i], wrong, *args[i + 1:])
