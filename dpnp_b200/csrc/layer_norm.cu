@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(WARP ? 256 : THREADS, WARP ? THREADS / 256 : 1
 }
 
 // dw, db = sum of the partial sums: 64 columns a block, 32 threads a pair of columns that take every 32nd
-// partial sum and are then added in order.
+// partial sum and are then added as a tree (one after the other they would lose what is small beside the first).
 template <class A, class W>
 __global__ void __launch_bounds__(1024) layer_norm_join_kernel(const A *part, int64_t slabs, int64_t n, W *dw, W *db)
 {
@@ -464,8 +464,19 @@ __global__ void __launch_bounds__(1024) layer_norm_join_kernel(const A *part, in
     buf[lane][col] = s;
     __syncthreads();
     if (lane > 0 || i >= 2 * n) return;
+    P t[4];
 #pragma unroll
-    for (int k = 1; k < 32; ++k) s = add2(s, buf[k][col]);
+    for (int k = 0; k < 4; ++k) {
+        P v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = buf[8 * k + u][col];
+#pragma unroll
+        for (int d = 4; d > 0; d >>= 1)
+#pragma unroll
+            for (int u = 0; u < d; ++u) v[u] = add2(v[u], v[u + d]);
+        t[k] = v[0];
+    }
+    s = add2(add2(t[0], t[1]), add2(t[2], t[3]));
     const auto put = [&](int64_t c, A v) { (c < n ? dw[c] : db[c - n]) = from_acc<W>(v); };
     put(i, s.x);
     put(i + 1, s.y);

@@ -1109,3 +1109,25 @@ def test_threads_with_rows_of_other_widths():
     assert not refused
     for (_, results, _), w in zip(jobs, want):
         assert all(np.array_equal(p, q) for p, q in zip(results(), w))
+
+
+@pytest.mark.parametrize("rows", [64, 512, 5000])
+@pytest.mark.parametrize("dt", ["f4", "f8"])
+def test_layer_norm_weight_gradients_add_their_parts_as_a_tree(dt, rows):
+    """One large term and many of 1, of which each would be lost in a sum of its own with the large one.  The rows
+    of a block are added one by one (at most rows / 64 + 1 of them here), the blocks' sums by 32 threads (at most
+    rows / 2048 + 1 each), and those as a tree of 5 levels: that many roundings of the total, 2^24 or 2^53, each of them
+    half a step of it at most, which is 1."""
+    import dpnp_b200 as dp
+
+    n = 1024
+    dy = np.ones((rows, n), dt)
+    dy[0] = 2.0**(24 if dt == "f4" else 53)
+    if rows == 64:
+        dy[32:] = 0
+    total = float(np.sum(dy[1:, 0]))
+    x, mean, rstd = np.ones((rows, n), dt), np.zeros(rows, dt), np.ones(rows, dt)
+    _, dw, db = dp.layer_norm_backward(dev(dy), dev(x), dev(mean), dev(rstd))
+    for g in (dw, db):
+        more = host(g) - dy[0, 0]                      # exact: both are above 2^24 (2^53)
+        assert np.all(np.abs(more - total) <= rows // 64 + 1 + rows // 2048 + 1 + 5), (more[0], total)
