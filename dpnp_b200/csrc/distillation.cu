@@ -7,10 +7,10 @@
 // A row without entries (padding, a prompt) has loss 0 and gradient 0, whatever its logits.
 // Where q is 0 (z = -inf, or every z of the row) and p is not, the loss is +inf; q counts as 0 in dz.
 //
-// log q = (z - max z) / T - log sum exp((z - max z) / T): the differences are taken before the
-// division, so that logits of the type's lowest value do not overflow.  The two statistics (max z, log
-// of the sum) are kept apart for the backward pass: their sum would lose log2 |max z| bits.  All of it
-// is float (double for float64 logits); each gradient is rounded once.
+// log q = (z - max z) / T - log sum exp((z - max z) / T): the differences are taken before the division, and the
+// terms of the loss are T (log p - log q), so that logits of the type's lowest value do not overflow.  The two
+// statistics (max z, log of the sum) are kept apart for the backward pass: their sum would lose log2 |max z| bits.
+// All of it is float (double for float64 logits); each gradient is rounded once.
 #include "row_ops.cuh"
 
 namespace dpb {
@@ -418,14 +418,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 4 : 6)
         if (rank == 0) {
             for (int i = lane; i < k; i += 32) {
                 if (part.teacher.at[i] < 0 || part.teacher.p[i] == 0) continue;
+                // T (log p - log q): the depth of the logit is not divided by T, which below 1 would take that of a
+                // logit of the type's lowest value out of range
                 const A v = part.at_teacher[i];
                 total += part.teacher.p[i] *
-                         (part.teacher.logp[i] - (v == -INFINITY ? A(-INFINITY) : (v - s.top) * inv_temp - log_sum));
+                         (v == -INFINITY ? A(INFINITY) : temp * (part.teacher.logp[i] + log_sum) + (s.top - v));
             }
             total = warp_fold(SumF(), total);
         }
         if (rank == 0 && lane == 0) {
-            if (loss) loss[r] = temp * temp * total;
+            if (loss) loss[r] = temp * total;
             if (stats) {
                 stats[2 * int64_t(r)] = s.top;
                 stats[2 * int64_t(r) + 1] = log_sum;

@@ -1131,3 +1131,21 @@ def test_layer_norm_weight_gradients_add_their_parts_as_a_tree(dt, rows):
     for g in (dw, db):
         more = host(g) - dy[0, 0]                      # exact: both are above 2^24 (2^53)
         assert np.all(np.abs(more - total) <= rows // 64 + 1 + rows // 2048 + 1 + 5), (more[0], total)
+
+
+@pytest.mark.parametrize("temp", [0.1, 0.5, 0.7, 1.0, 2.0])
+@pytest.mark.parametrize("dt", TYPES)
+def test_distillation_at_columns_of_the_lowest_value(dt, temp):
+    """A teacher's entry at a masked column: the loss is p T times the mask's depth, a number of the type, although the
+    depth over T is not when T is below 1."""
+    rng = np.random.default_rng(13)
+    for rows, vocab, k in ((6, 40, 3), (4, 5001, 5), (3, 70000, 4)):
+        z = rng.normal(0, 2, (rows, vocab)).astype(dt)
+        z[:, ::7] = np.finfo(dt).min
+        idx = 7 * np.stack([rng.choice(vocab // 7, k, replace=False) for _ in range(rows)]).astype("i4")
+        idx[:, 1:] += 1                                 # the other entries are at columns that are not masked
+        t = rng.normal(0, 1, (rows, k)).astype(ACC[dt])
+        t[:, 0] -= 2 * temp
+        loss, grad, _ = run_distil(z, t, idx, temp)
+        if temp <= 1:                                   # p T < 1; its value is compared in run_distil
+            assert np.isfinite(loss).all()
