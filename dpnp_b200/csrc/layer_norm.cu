@@ -561,8 +561,11 @@ static bool launch_forward(const NormArgs &a, int64_t accesses, cudaStream_t s)
 // accesses go to a warp (524288 x 256 float16: 104 us against 132 us), rows of more than 2048 take four
 // accesses a thread and one row, with the weights in shared memory where they fit (4194 x 16001 float32: 103 us, 165 us
 // from the caches).  So do shifted rows of more than 1024 accesses where two blocks fit an SM (16380 x 4097 float32:
-// 94 us, 134 us with two accesses and 544 threads), and those for which one warp is enough then (222953 x 301 float32:
-// 129 us against 174).  False: the row is longer than 4096 accesses.
+// 94 us, 134 us with two accesses and 544 threads), and those of 65 to 128 accesses, for which one warp is enough then:
+// 0.74 to 0.78 of the time of two warps and two rows up to 96 accesses and 0.83 to 0.97 above (111476 x 301 float32: 65 us
+// against 86; 74565 x 225 float64: 55 against 66; 77582 x 865 float16: 86 against 90).  float16 rows with float32 weights
+// are at 0.92 up to 96 accesses and at 1.12 above, where they stay with two warps.  False: the row is longer than 4096
+// accesses.
 template <class T, class W, int VEC, bool SHIFT> static bool run_rows(const NormArgs &a, cudaStream_t s)
 {
     const int64_t nv = ceil_div(a.n + (SHIFT ? VEC - 1 : 0), VEC);
@@ -575,7 +578,8 @@ template <class T, class W, int VEC, bool SHIFT> static bool run_rows(const Norm
         constexpr int keep = is_half_v<T> ? kShared : kRegisters;
         if (nv <= 32) return launch_forward<T, W, VEC, 1, true, 2, 3, kRegisters, SHIFT>(a, nv, s);
         const int64_t four = ceil_div(ceil_div(nv, 4), 32) * 32 * 4 * VEC * (sizeof(T) + 2 * sizeof(W));   // bytes with four accesses
-        if (SHIFT && ((nv > 64 && nv <= 80) || (nv > 1024 && nv <= 2048 && four <= 112 * 1024)))
+        constexpr int one_warp = sizeof(W) > sizeof(T) ? 96 : 128;
+        if (SHIFT && ((nv > 64 && nv <= one_warp) || (nv > 1024 && nv <= 2048 && four <= 112 * 1024)))
             return launch_forward<T, W, VEC, 4, false, 1, 1, kShared, SHIFT>(a, nv, s);
         if (nv <= 2048) return launch_forward<T, W, VEC, 2, false, 2, 1, keep, SHIFT>(a, nv, s);
         if (nv <= 4096 && four <= 224 * 1024) return launch_forward<T, W, VEC, 4, false, 1, 1, kShared, SHIFT>(a, nv, s);

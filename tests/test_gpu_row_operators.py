@@ -1149,3 +1149,17 @@ def test_distillation_at_columns_of_the_lowest_value(dt, temp):
         loss, grad, _ = run_distil(z, t, idx, temp)
         if temp <= 1:                                   # p T < 1; its value is compared in run_distil
             assert np.isfinite(loss).all()
+
+
+@pytest.mark.parametrize("dt,wt,widths", [("f4", "f4", (253, 257, 333, 381, 385, 401, 509, 513)), ("f8", "f8", (127, 129, 165, 191, 193, 255, 257)),
+                                          ("f2", "f2", (505, 513, 737, 761, 769, 865, 1017, 1025)),
+                                          ("f2", "f4", (505, 513, 737, 761, 769, 865, 1017, 1025))])
+def test_layer_norm_of_shifted_rows_of_one_warp(dt, wt, widths):
+    """Rows off the 16-byte grid on both sides of the lengths between which a warp takes a row by four accesses."""
+    import dpnp_b200 as dp
+
+    for n in widths:
+        for rows in (1, 9, 3001):
+            x, w, b, _ = norm_data(rows, n, dt, wt, n + rows)
+            y, mean, rstd = dp.layer_norm(dev(x), dev(w), dev(b), return_stats=True)
+            check_norm(x, w, b, 1e-5, host(y), host(mean), host(rstd))
