@@ -186,11 +186,20 @@ struct BlockInfo {
 static std::unordered_map<void *, BlockInfo> g_blocks;
 static std::mutex g_blocks_mutex;
 
+// While a stream is captured, calls that may synchronise are refused to the thread; those between the two ends of
+// this object are not part of the capture and are let through.
+struct OutsideCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 static int configure_pool(int dev)
 {
     if (g_pool[dev].configured.load(std::memory_order_acquire)) return DPB_OK;
     std::lock_guard<std::mutex> lock(g_pool_mutex);
     if (g_pool[dev].configured.load(std::memory_order_relaxed)) return DPB_OK;
+    OutsideCapture outside;   // (a program's first scratch may be needed within a capture)
     cudaMemPool_t pool;
     DPB_CUDA_TRY(cudaDeviceGetDefaultMemPool(&pool, dev));
     // Keep freed blocks cached instead of returning them to the driver at

@@ -1163,3 +1163,42 @@ def test_layer_norm_of_shifted_rows_of_one_warp(dt, wt, widths):
             x, w, b, _ = norm_data(rows, n, dt, wt, n + rows)
             y, mean, rstd = dp.layer_norm(dev(x), dev(w), dev(b), return_stats=True)
             check_norm(x, w, b, 1e-5, host(y), host(mean), host(rstd))
+
+
+FIRST_CALLS_CAPTURED = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import dpnp_b200 as dp
+from test_gpu_row_operators import RESULTS, _arrays, _step, _tensors, _views
+
+t = _tensors(torch, 3, tokens=40, vocab=50, n=8192, k=300)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    _step(dp, _views(dp, t, dp.StreamQueue(0, stream=torch.cuda.current_stream().cuda_stream)))
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+got = {{k: t[k].clone() for k in RESULTS}}
+for k in RESULTS:
+    t[k].zero_()
+torch.cuda.synchronize()
+_step(dp, _arrays(dp, t, dp.StreamQueue(0, stream=torch.cuda.current_stream().cuda_stream)))
+torch.cuda.synchronize()
+assert all(torch.equal(t[k], got[k]) for k in RESULTS)
+"""
+
+
+def test_first_calls_of_a_program_within_a_capture():
+    """A program that captures its step without a pass before: what the library sets up once a device, the pool of
+    the scratch and the kernels' shared memory, is set up during the capture."""
+    import os
+    import subprocess
+    import sys
+
+    pytest.importorskip("torch")
+    tests = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALLS_CAPTURED.format(root=os.path.dirname(tests), tests=tests)
+    proc = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert proc.returncode == 0, proc.stderr[-3000:]
