@@ -157,7 +157,9 @@ template <class A> struct Teacher {
             logp[i] = at[i] >= 0 ? (logp[i] - best) * inv_temp - log_sum : A(0);
         }
     }
-    // All the weight on the column of entry i; false when an earlier entry has the same column.
+    // All the weight on the column of entry i; false when an earlier entry has the same column.  K comparisons an entry:
+    // little up to some hundred entries, the greater part of the time at 1024 (4096 x 128000 float16, gradient alone: 330 us
+    // with 64 entries, 383 with 256, 3091 with 1024; with the loss 393, 621 and 5960).
     DPB_D bool first_of_column(int i, int k, A &weight) const
     {
         bool first = true;
@@ -317,13 +319,16 @@ template <class T, class I> struct RowPart {
 // --------------------------------------------------------------------------------- loss, and loss and gradient
 // A cluster of 1 to 8 blocks takes a row: every block streams its part (largest value and sum of exponentials, both per
 // thread), the blocks exchange their sums through distributed shared memory, and (GRAD) read their parts again,
-// from the second-level cache, for the gradient: the logits cross the memory once.  The clusters that run at a
-// time hold 30 to 60 MB, which the cache keeps.  4096 x 128000 float16 takes 400 us (0.80 of the copy rate); the
+// from the second-level cache, for the gradient: with parts of 64 KiB the clusters that run at a time hold 30 to 60 MB,
+// which the cache keeps, and the logits cross the memory once.  That holds for rows of up to 512 KiB.  The parts of longer
+// rows grow, and the second reading misses: 1024 x 131072 float32 reads 1.04 times the logits (197 us, 0.83 of the copy
+// rate), 1024 x 150001 1.20 times (242 us, 0.78), 512 x 300000 1.98 times (307 us, 0.61).  float64 is bound by its
+// exponentials (512 x 150001: loss 192 us, gradient 252 us, both 428 us).  4096 x 128000 float16 takes 400 us (0.80); the
 // parts kept in shared memory instead, by copies that run ahead, 487 us, because few threads fit beside them; clusters
 // that stay and fetch the next row's teacher ahead, 766 us, because they read and write in step.  What a block waits for
 // beside its part counts as much as the bytes: the first logits are fetched with the teacher's entries, the student's
 // logits at their columns arrive while the part is streamed, and one warp forms the probabilities and the loss while the
-// others go on (418 us with these one after the other; 1024 x 150001 float32: 288, now 264).
+// others go on (418 us with these one after the other; 1024 x 150001 float32 timed one by one: 288, now 264).
 //
 // Two exponentials an element: at float16 and the copy rate that is 3.3e12 a second, three quarters of what the
 // special function units give; the rest of the arithmetic is done in pairs to stay out of their way.
